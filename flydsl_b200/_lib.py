@@ -24,6 +24,7 @@ DT_FP8, DT_INT8, DT_FP16, DT_BF16 = range(4)
 OUT_BF16, OUT_FP16, OUT_F32 = range(3)
 EPI_NONE, EPI_BIAS, EPI_BIAS_RELU, EPI_BIAS_SILU, EPI_BIAS_GELU = range(5)
 SRC_ROW_MAJOR, SRC_MFMA_16x16 = range(2)
+ROWQ_NONE, ROWQ_FP8, ROWQ_INT8, ROWQ_MXFP8 = range(4)
 MOE_QUANT_MAX_K = 16384
 
 IN_DTYPES = {"fp8": DT_FP8, "int8": DT_INT8, "fp16": DT_FP16, "bf16": DT_BF16}
@@ -49,6 +50,9 @@ SIGNATURES = {
         [ctypes.POINTER(_vp), _i, _i, ctypes.c_longlong, ctypes.c_longlong, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
     ),
     "flyb200_pertoken_quant": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "flyb200_rmsnorm_quant": (_i, [_vp] * 6 + [_i, _i] + [ctypes.c_longlong] * 3 + [ctypes.c_float, _i, _i, _i, _vp]),
+    "flyb200_silu_mul_quant": (_i, [_vp, _vp, _vp, _i, _i, ctypes.c_longlong, _i, _i, _vp]),
+    "flyb200_gemv_w4a16": (_i, [_vp] * 6 + [_i] * 6 + [_vp]),
     "flyb200_shuffle_weight": (_i, [_vp, _vp, _i, _i, _i, _i, _vp]),
     "flyb200_unshuffle_weight": (_i, [_vp, _vp, _i, _i, _i, _vp]),
     "flyb200_pair_width": (_i, [_i, _i, _i, _i, _i, _i]),

@@ -37,6 +37,8 @@ SOURCES = [
     "flyb200_decode2.cu",
     "flyb200_moe.cu",
     "flyb200_mx.cu",
+    "flyb200_rowops.cu",
+    "flyb200_w4.cu",
 ]
 HEADERS = [
     "ptx.cuh",

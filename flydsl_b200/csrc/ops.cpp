@@ -54,6 +54,15 @@ struct Args {
     }
     return x;
   }
+  double real() {
+    const double x = i < n ? PyFloat_AsDouble(v[i]) : -1.0;
+    ++i;
+    if (x == -1.0) {  // also what an error returns; no argument is -1
+      PyErr_Clear();
+      ok = false;
+    }
+    return x;
+  }
   int i32() {
     const long long x = integer();
     if (x < INT_MIN || x > INT_MAX) ok = false;
@@ -141,6 +150,138 @@ PyObject* pertoken_quant(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     rc = flyb200_pertoken_quant(ptr(y), as<float>(s), ptr(x), static_cast<int>(x.numel() / k), static_cast<int>(k), in, qd, stream_of(x));
   }
   return rc ? code(rc) : tuple({y, s});
+  END_HANDLE_TH_ERRORS
+}
+
+// Rows of a tensor [..., K]: their number and the elements from one to the next; false where they do not lie at equal distances.
+bool rows_of(const at::Tensor& t, long long& rows, long long& stride) {
+  const int64_t d = t.dim(), k = d > 0 ? t.size(-1) : 0;
+  if (k <= 0 || k >= (1ll << 30) || t.numel() == 0 || (k > 1 && t.stride(-1) != 1)) return false;
+  rows = t.numel() / k;
+  stride = -1;
+  long long expect = 0;
+  for (int64_t i = d - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (stride < 0) stride = t.stride(i);
+    else if (t.stride(i) != expect) return false;
+    expect = t.stride(i) * t.size(i);
+  }
+  if (stride < 0) stride = k;
+  return stride >= k && rows < (1ll << 31);
+}
+struct RowOutputs {
+  at::Tensor y, scale;
+};
+RowOutputs row_outputs(const at::Tensor& x, int64_t width, int quant) {
+  c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = width;
+  RowOutputs o;
+  o.y = at::empty(shape, quant == FLYB200_ROWQ_NONE ? x.options() : x.options().dtype(quant == FLYB200_ROWQ_INT8 ? at::kChar : at::kFloat8_e4m3fn));
+  if (quant == FLYB200_ROWQ_MXFP8) {
+    shape.back() = width / 32;
+    o.scale = at::empty(shape, x.options().dtype(at::kByte));
+  } else if (quant != FLYB200_ROWQ_NONE) {
+    shape.back() = 1;
+    o.scale = at::empty(shape, x.options().dtype(at::kFloat));
+  }
+  return o;
+}
+
+// rmsnorm_quant(x, weight, residual | None, residual_out | None, eps, quant) -> (y, scale | None, residual_out | None).
+// residual_out given: only the residual itself, updated in place.
+PyObject* rmsnorm_quant(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{argv, n};
+  const at::Tensor &x = a.tensor(), &w = a.tensor(), &res = a.tensor_or_none(), &out = a.tensor_or_none();
+  const double eps = a.real();
+  const int quant = a.i32();
+  if (!a.done() || !runs_eagerly(argv[0], true) || !runs_eagerly(argv[1], true)) return none();
+  if (!x.is_cuda() || x.layout() != at::kStrided || x.dim() < 1 || quant < FLYB200_ROWQ_NONE || quant > FLYB200_ROWQ_MXFP8) return none();
+  const int in = input_code(x);
+  long long rows = 0, stride = 0, r_stride = 0, h_stride = 0;
+  if (in < 0 || !rows_of(x, rows, stride)) return none();
+  const int64_t k = x.size(-1);
+  if (!plain(w) || w.dim() != 1 || w.numel() != k || w.device() != x.device() || (w.scalar_type() != x.scalar_type() && w.scalar_type() != at::kFloat))
+    return none();
+  if (quant == FLYB200_ROWQ_MXFP8 && k % 32 != 0) return none();
+  if (res.defined()) {
+    if (!runs_eagerly(argv[2], true) || !res.is_cuda() || res.layout() != at::kStrided || res.device() != x.device() ||
+        res.scalar_type() != x.scalar_type() || res.sizes() != x.sizes() || !rows_of(res, rows, r_stride))
+      return none();
+  }
+  if (out.defined()) {
+    if (!res.defined() || !plain(out) || !plain(res) || !plain(x) || out.data_ptr() != res.data_ptr() || out.sizes() != res.sizes() ||
+        out.scalar_type() != res.scalar_type() || !runs_eagerly(argv[3], true))
+      return none();
+    const char *h0 = static_cast<const char*>(ptr(out)), *x0 = static_cast<const char*>(ptr(x)), *w0 = static_cast<const char*>(ptr(w));
+    const size_t bytes = out.nbytes();
+    if ((x0 < h0 + bytes && h0 < x0 + bytes && x0 != h0) || (w0 < h0 + bytes && h0 < w0 + w.nbytes())) return none();
+  }
+  at::Tensor h;
+  RowOutputs o;
+  int rc;
+  {
+    NoGil g;
+    const c10::cuda::CUDAGuard dev(x.device());
+    o = row_outputs(x, k, quant);
+    if (res.defined()) {
+      h = out.defined() ? out : at::empty(x.sizes(), x.options());
+      h_stride = k;
+    }
+    rc = flyb200_rmsnorm_quant(ptr(o.y), ptr(o.scale), ptr(h), ptr(x), ptr(res), ptr(w), static_cast<int>(rows), static_cast<int>(k), stride,
+                               r_stride, h_stride, static_cast<float>(eps), in, w.scalar_type() == at::kFloat, quant, stream_of(x));
+  }
+  return rc ? code(rc) : tuple({o.y, o.scale, h});
+  END_HANDLE_TH_ERRORS
+}
+
+// silu_mul_quant(x, quant) -> (y, scale | None)
+PyObject* silu_mul_quant(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{argv, n};
+  const at::Tensor& x = a.tensor();
+  const int quant = a.i32();
+  if (!a.done() || !runs_eagerly(argv[0], true) || !x.is_cuda() || x.layout() != at::kStrided || x.dim() < 1 || quant < FLYB200_ROWQ_NONE ||
+      quant > FLYB200_ROWQ_MXFP8)
+    return none();
+  const int in = input_code(x);
+  long long rows = 0, stride = 0;
+  if (in < 0 || !rows_of(x, rows, stride) || x.size(-1) % 2 != 0) return none();
+  const int64_t inter = x.size(-1) / 2;
+  if (quant == FLYB200_ROWQ_MXFP8 && inter % 32 != 0) return none();
+  RowOutputs o;
+  int rc;
+  {
+    NoGil g;
+    const c10::cuda::CUDAGuard dev(x.device());
+    o = row_outputs(x, inter, quant);
+    rc = flyb200_silu_mul_quant(ptr(o.y), ptr(o.scale), ptr(x), static_cast<int>(rows), static_cast<int>(inter), stride, in, quant, stream_of(x));
+  }
+  return rc ? code(rc) : tuple({o.y, o.scale});
+  END_HANDLE_TH_ERRORS
+}
+
+// w4_gemv(c, a, q, scale, zero | None, bias | None, M, N, K, group, dtype, epilogue, stream) -> code
+PyObject* w4_gemv(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{argv, n};
+  const at::Tensor &c = a.tensor(), &x = a.tensor(), &q = a.tensor(), &scale = a.tensor(), &zero = a.tensor_or_none(), &bias = a.tensor_or_none();
+  const int M = a.i32(), N = a.i32(), K = a.i32(), group = a.i32(), dtype = a.i32(), epi = a.i32();
+  const long long s = a.integer();
+  if (!a.done() || M <= 0 || N <= 0 || K <= 0 || group <= 0) return none();
+  const at::ScalarType t = dtype == FLYB200_DT_FP16 ? at::kHalf : at::kBFloat16;
+  const long long m = M, nn = N, k = K, groups = nn * (k / group);
+  auto fits = [&](const at::Tensor& v, long long least) { return plain(v) && v.scalar_type() == t && v.numel() >= least && v.device() == c.device(); };
+  if (!fits(c, m * nn) || !fits(x, m * k) || !fits(scale, groups) || !bytes(q, nn * k / 2) || q.device() != c.device()) return none();
+  if (zero.defined() && (!plain(zero) || zero.scalar_type() != at::kByte || zero.numel() < groups || zero.device() != c.device())) return none();
+  if (epi != FLYB200_EPI_NONE && !fits(bias, nn)) return none();
+  int rc;
+  {
+    NoGil g;
+    const c10::cuda::CUDAGuard dev(c.device());
+    rc = flyb200_gemv_w4a16(ptr(c), ptr(x), ptr(q), ptr(scale), ptr(zero), ptr(bias), M, N, K, group, dtype, epi, handle(s));
+  }
+  return code(rc);
   END_HANDLE_TH_ERRORS
 }
 
@@ -402,7 +543,7 @@ PyObject* moe_layer(PyObject*, PyObject* const* argv, Py_ssize_t n) {
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(pertoken_quant), FAST(gemm_a8w8), FAST(eager), FAST(mx_quant), FAST(mx_scale_image), FAST(mx_gemm),
+PyMethodDef methods[] = {FAST(pertoken_quant), FAST(rmsnorm_quant), FAST(silu_mul_quant), FAST(w4_gemv), FAST(gemm_a8w8), FAST(eager), FAST(mx_quant), FAST(mx_scale_image), FAST(mx_gemm),
                          FAST(moe_sort),       FAST(moe_stage), FAST(moe_layer), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "flyb200_ops", "Host path of the operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -16,7 +16,7 @@ def _left_to_the_caller(*args):
     return None
 
 
-pertoken_quant = mx_quant = mx_scale_image = mx_gemm = moe_sort = moe_layer = _left_to_the_caller
+rmsnorm_quant = silu_mul_quant = w4_gemv = pertoken_quant = mx_quant = mx_scale_image = mx_gemm = moe_sort = moe_layer = _left_to_the_caller
 
 
 def _ptr(t):

@@ -206,6 +206,46 @@ int flyb200_unshuffle_weight(void* dst, const void* src, int N, int K, int elem_
 int flyb200_pertoken_quant(void* y, float* scale, const void* x, int rows, int K, int x_dtype, int quant_dtype,
                            void* stream);
 
+/* ---- row operators: what feeds the quantised products ----
+ * The form of their output, of values v held in fp32:
+ *   NONE   v rounded to the type of x; scale = NULL
+ *   FP8, INT8   y = nearest(v / s) (ties to even), scale[rows] fp32 = rowmax|v| * (1/qmax) with 0 -> 1, qmax 448 / 127;
+ *          NaN -> 0 and +-Inf -> +-qmax beforehand, as in flyb200_pertoken_quant (which truncates int8, as the reference does)
+ *   MXFP8  E4M3 codes and one E8M0 byte per 32 values, scale[rows, width / 32], as flyb200_mx_quant
+ * y has rows of `width` elements without gaps.  Strides are in elements, those of x and the residuals in their own type.
+ * x_dtype: 0 = fp32, 1 = fp16, 2 = bf16.  Any width and stride runs; rows whose width, strides and addresses are multiples
+ * of 16 bytes are read in vectors.  Outputs must not overlap inputs, but residual_out may be x or residual itself. */
+#define FLYB200_ROWQ_NONE 0
+#define FLYB200_ROWQ_FP8 1
+#define FLYB200_ROWQ_INT8 2
+#define FLYB200_ROWQ_MXFP8 3
+
+/* Residual addition, root-mean-square norm and quantisation:
+ *   h = x + residual, rounded to the type of x (h = x without a residual), residual_out = h
+ *   v = h * weight / sqrt(mean(h^2) + eps), statistics and v in fp32
+ * x, residual, residual_out [rows, K] of one type; weight [K] of that type, or fp32 with weight_f32.  residual and
+ * residual_out are both NULL or both given.  MXFP8: K a multiple of 32. */
+int flyb200_rmsnorm_quant(void* y, void* scale, void* residual_out, const void* x, const void* residual, const void* weight,
+                          int rows, int K, long long x_stride, long long residual_stride, long long residual_out_stride,
+                          float eps, int x_dtype, int weight_f32, int quant, void* stream);
+
+/* Gated activation and quantisation: x[rows, 2 * inter], of every row the gate values first;
+ * v = gate / (1 + exp(-gate)) * up in fp32.  MXFP8: inter a multiple of 32. */
+int flyb200_silu_mul_quant(void* y, void* scale, const void* x, int rows, int inter, long long x_stride, int x_dtype, int quant,
+                           void* stream);
+
+/* ---- products of few tokens on 4-bit weights with a scale per group of inputs ----
+ * c[m, n] = epilogue(sum over groups g of scale[n, g] * sum over k in g of (q[n, k] - z[n, g]) * a[m, k])
+ *   a        [M, K] and c [M, N] row-major, dtype FLYB200_DT_BF16 or FLYB200_DT_FP16; rows of c past M are never written
+ *   q        [N, K / 2] bytes, row-major, two codes 0..15 per byte: input 2i in the low half of byte i
+ *   scale    [N, K / group] of the type of a
+ *   zero     [N, K / group] bytes 0..15, or NULL: 8 everywhere (codes are then signed numbers plus 8)
+ *   bias     [N] of the type of a; NULL when epilogue == FLYB200_EPI_NONE
+ * Code minus zero point is an exact number in the multiply; sums over a group are fp32 and the scale multiplies them in fp32.
+ * Requirements: group 32, 64 or 128, K a multiple of it; a and q 16-byte aligned. */
+int flyb200_gemv_w4a16(void* c, const void* a, const void* q, const void* scale, const void* zero, const void* bias, int M, int N,
+                       int K, int group, int dtype, int epilogue, void* stream);
+
 /* 1 when (N, K, elem_bytes) can be preshuffled into the B200 image, else 0.
  * A pure function of its arguments: the helper and the GEMM evaluate the same
  * predicate because the `is_shuffled` attribute does not survive the flat views
