@@ -39,6 +39,7 @@ SOURCES = [
     "flyb200_mx.cu",
     "flyb200_rowops.cu",
     "flyb200_w4.cu",
+    "flyb200_w4_wide.cu",
 ]
 HEADERS = [
     "ptx.cuh",
