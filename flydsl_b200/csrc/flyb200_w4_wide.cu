@@ -23,12 +23,10 @@ namespace {
 
 constexpr int ROWS = 128;         // of weights in a block
 constexpr int STAGE_K = 256;      // inputs of a stage of the ring: 128 bytes of a row of codes
-constexpr int HALF_K = 128;       // inputs decoded at a time by one of the two groups of decoding warps
+constexpr int HALF_K = 128;       // inputs that a group of decoding warps takes at a time
 constexpr int HALF_COLS = HALF_K / 2;  // columns of tensor memory that they take
-constexpr int A_SLOTS = 4;
+constexpr int SLOTS = 4;          // of them
 constexpr uint32_t TMEM_COLS = 512;
-// warps 0-3: sums (one per quarter of the rows), 4-7 and 8-11: decoding, 12: loads, 13: multiplies
-constexpr int THREADS = 14 * 32;
 
 struct WideParams {
   void* c;
@@ -43,14 +41,19 @@ struct WideParams {
 
 template <int NT, int G>
 struct Wide {
+  // Warps: sums (a thread has a row and up to 32 tokens), one of loads, one of multiplies, two of nothing, groups of four that decode.
+  static constexpr int SUM_COLS = NT > 32 ? 32 : NT, SUM_WARPS = 4 * NT / SUM_COLS;
+  static constexpr int LOAD_WARP = SUM_WARPS, MULTIPLY_WARP = SUM_WARPS + 1, DECODE_WARP = SUM_WARPS + 4;
+  static constexpr int DECODERS = NT > 32 ? 3 : 4;
+  static constexpr int THREADS = 32 * (DECODE_WARP + 4 * DECODERS);
   static constexpr int CODES = ROWS * 128, TOKENS = 4 * NT * 128;  // bytes of a stage
   static constexpr int STAGE = CODES + TOKENS;
   static constexpr int RED = NT * ROWS * 4;
   static constexpr int STAGES = (226 * 1024 - RED - 1024) / STAGE > 8 ? 8 : (226 * 1024 - RED - 1024) / STAGE;
   static constexpr int OFF_RED = STAGES * STAGE, OFF_MISC = OFF_RED + RED, BYTES = OFF_MISC + 512;
   static constexpr int GROUPS = HALF_K / G;  // of a half stage, each with NT columns of sums
-  static constexpr int FIT = (static_cast<int>(TMEM_COLS) - A_SLOTS * HALF_COLS) / (GROUPS * NT);
-  static constexpr int SETS = FIT > 4 ? 4 : FIT;  // of sums of a half stage
+  static constexpr int FIT = (static_cast<int>(TMEM_COLS) - SLOTS * HALF_COLS) / (GROUPS * NT);
+  static constexpr int SETS = FIT > SLOTS ? SLOTS : FIT;  // of sums of a half stage
   static_assert(SETS >= 1 && STAGES >= 3 && BYTES <= 227 * 1024, "shared and tensor memory");
 };
 
@@ -126,21 +129,23 @@ __device__ __forceinline__ float wide_activation(float v, int epi) {
 }
 
 // Roles meet at barriers in shared memory, each wait of bounded length:
-//   full[stage]   codes and tokens of a stage have landed            empty[stage]  decoded (8 warps) and multiplied (commit)
-//   afull[slot]   half a stage of numbers is in tensor memory (4)    aempty[slot]  multiplied (commit)
-//   dfull[set]    sums of half a stage (commit)                      dempty[set]   added to the result (4 warps)
+//   full[stage]   codes and tokens of a stage have landed
+//   empty[stage]  multiplied (commit), so decoded too
+//   ready[slot]   half a stage of numbers is in tensor memory (4 warps), and the sums of the half SETS before it have left (SUM_WARPS)
+//   done[slot]    multiplied (commit): the sums are there, the numbers may go
+// The warp of multiplies sets the pace where it has more to do than this: a wait costs it about 120 cycles, a commit 100
+// (half a stage in 900 cycles with three of each, 540 with one and a half).
 template <typename T, int G, int NT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     gemv_w4_wide_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_tokens, const WideParams p) {
   using L = Wide<NT, G>;
-  constexpr int GROUPS = L::GROUPS;
+  constexpr int GROUPS = L::GROUPS, THREADS = L::THREADS, SETS = L::SETS;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const uint32_t full = base + L::OFF_MISC + 16, empty = full + 8 * L::STAGES, afull = empty + 8 * L::STAGES, aempty = afull + 8 * A_SLOTS,
-                 dfull = aempty + 8 * A_SLOTS, dempty = dfull + 8 * 4;
+  const uint32_t full = base + L::OFF_MISC + 16, empty = full + 8 * L::STAGES, ready = empty + 8 * L::STAGES, done = ready + 8 * SLOTS;
   if ((base & 1023u) != 0) {  // the same in all blocks: nobody waits for this one
     if (threadIdx.x == 0) atomicCAS(p.status, 0, ST_SMEM_ALIGN);
     return;
@@ -148,15 +153,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::STAGES; ++s) {
       mbar_init(full + 8 * s, 1);
-      mbar_init(empty + 8 * s, 9);
+      mbar_init(empty + 8 * s, 1);
     }
-    for (int s = 0; s < A_SLOTS; ++s) {
-      mbar_init(afull + 8 * s, 4);
-      mbar_init(aempty + 8 * s, 1);
-    }
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(dfull + 8 * s, 1);
-      mbar_init(dempty + 8 * s, 4);
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(ready + 8 * s, 4 + L::SUM_WARPS);
+      mbar_init(done + 8 * s, 1);
     }
     abort_flag[0] = 0;
     abort_flag[1] = 0;
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     prefetch_tensormap(&tm_codes);
     prefetch_tensormap(&tm_tokens);
   }
-  if (warp == 13) {
+  if (warp == L::MULTIPLY_WARP) {
     tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
     tmem_relinquish();
   }
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t d0 = tmem, a0 = tmem + TMEM_COLS - A_SLOTS * HALF_COLS;
+  const uint32_t d0 = tmem, a0 = tmem + TMEM_COLS - SLOTS * HALF_COLS;
   pdl_wait<>();  // nothing in global memory is touched before this
   pdl_trigger();
 
@@ -183,9 +184,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int n_groups = p.K / G;
   const int row = warp % 4 * 32 + lane;  // of sums and decoding warps
   const uint32_t quarter = static_cast<uint32_t>(warp % 4 * 32) << 16;
-  float acc[NT];
+  float acc[L::SUM_COLS];
 
-  if (warp == 12) {
+  if (warp == L::LOAD_WARP) {
     // ---- loads ----
     const bool issuer = elect_one();
     const uint64_t once = l2_policy_evict_first(), kept = l2_policy_evict_last();
@@ -217,15 +218,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_wait(full + 8 * s, ph, abort_flag + 1);
       }
     }
-  } else if (warp == 13) {
+  } else if (warp == L::MULTIPLY_WARP) {
     // ---- multiplies ----
     const bool issuer = elect_one();
     constexpr uint32_t idesc = umma_idesc(1, Wide16<T>::FORMAT, ROWS, NT);
     int stage = 0, slot = 0, set = 0;
-    uint32_t phase = 0, a_phase = 0, d_phase = 0;
+    uint32_t phase = 0, slot_phase = 0;
     for (int h = 0; h < halves; ++h) {
-      if (((h & 1) == 0 && !mbar_wait_warp(full + 8 * stage, phase, abort_flag)) || !mbar_wait_warp(dempty + 8 * set, d_phase ^ 1u, abort_flag) ||
-          !mbar_wait_warp(afull + 8 * slot, a_phase, abort_flag)) {
+      if (((h & 1) == 0 && !mbar_wait_warp(full + 8 * stage, phase, abort_flag)) || !mbar_wait_warp(ready + 8 * slot, slot_phase, abort_flag)) {
         report_failure(p.status, ST_TIMEOUT, abort_flag);
         break;
       }
@@ -237,48 +237,47 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint64_t bdesc = umma_desc_sw128_kmajor(tokens + (k / 4) * NT * 128) + static_cast<uint64_t>((k % 4) * 2);
           umma_ts_f16(d0 + (set * GROUPS + k * 16 / G) * NT, a0 + slot * HALF_COLS + k * 8, bdesc, idesc, k * 16 % G != 0 ? 1u : 0u);
         }
-        umma_commit(aempty + 8 * slot);
-        umma_commit(dfull + 8 * set);
+        umma_commit(done + 8 * slot);
         if (h & 1) umma_commit(empty + 8 * stage);
       }
       if ((h & 1) && ++stage == L::STAGES) stage = 0, phase ^= 1u;
-      if (++slot == A_SLOTS) slot = 0, a_phase ^= 1u;
-      if (++set == L::SETS) set = 0, d_phase ^= 1u;
+      if (++slot == SLOTS) slot = 0, slot_phase ^= 1u;
+      if (++set == SETS) set = 0;
     }
-  } else if (warp >= 4) {
-    // ---- decoding: warps 4-7 the first, 8-11 the second half of every stage ----
-    const int mine = (warp - 4) / 4;
+  } else if (warp >= L::DECODE_WARP) {
+    // ---- decoding: group i takes the halves i, i + DECODERS, ...  The codes of the next one are read while the numbers of this one
+    // are on their way to tensor memory. ----
     const size_t zero_row = static_cast<size_t>(min(n0 + row, p.N - 1)) * n_groups;
-    int stage = 0, slot = mine;
-    uint32_t phase = 0, a_phase = 0;
+    int h = (warp - L::DECODE_WARP) / 4, stage = h / 2, slot = h % SLOTS;
+    uint32_t phase = 0, slot_phase = 0;
     uint8_t next[GROUPS];
-    auto load_zeros = [&](int s) {
+    auto load_zeros = [&](int half) {
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
         next[j] = 8;
-        if (p.zero) next[j] = __ldg(p.zero + zero_row + min((2 * s + mine) * GROUPS + j, n_groups - 1));
+        if (p.zero) next[j] = __ldg(p.zero + zero_row + min((2 * s0 + half) * GROUPS + j, n_groups - 1));
       }
     };
-    if (s0 < s1) load_zeros(s0);
-    for (int s = s0; s < s1; ++s) {
+    uint4 w[4];
+    auto read_codes = [&]() {
+      if (!mbar_wait_warp(full + 8 * stage, phase, abort_flag)) return false;
+      const uint32_t at = base + stage * L::STAGE + row * 128;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = ld_smem_v4(at + ((((h & 1) * 4 + i) ^ (row & 7)) << 4));
+      return true;
+    };
+    bool ok = true;
+    if (h < halves) {
+      load_zeros(h);
+      ok = read_codes();
+    }
+    while (h < halves && ok) {
       uint32_t offset[GROUPS];
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) offset[j] = (Wide16<T>::MAGIC + (next[j] & 15u)) * 0x10001u;
-      if (s + 1 < s1) load_zeros(s + 1);
-      if (!mbar_wait_warp(full + 8 * stage, phase, abort_flag)) {
-        if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
-        break;
-      }
-      uint4 w[4];
-      const uint32_t at = base + stage * L::STAGE + row * 128;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = ld_smem_v4(at + (((mine * 4 + i) ^ (row & 7)) << 4));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + 8 * stage);
-      if (!mbar_wait_warp(aempty + 8 * slot, a_phase ^ 1u, abort_flag)) {
-        if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
-        break;
-      }
+      const int then = h + L::DECODERS;
+      if (then < halves) load_zeros(then);
+      if (!(ok = mbar_wait_warp(done + 8 * slot, slot_phase ^ 1u, abort_flag))) break;
       tc_fence_after();
       const uint32_t dst = a0 + quarter + slot * HALF_COLS;
 #pragma unroll
@@ -292,61 +291,62 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         tmem_st_x32(dst + part * 32, d);
       }
+      const uint32_t written = ready + 8 * slot;
+      stage += then / 2 - h / 2;
+      if (stage >= L::STAGES) stage -= L::STAGES, phase ^= 1u;
+      slot += L::DECODERS;
+      if (slot >= SLOTS) slot -= SLOTS, slot_phase ^= 1u;
+      h = then;
+      if (h < halves) ok = read_codes();
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(afull + 8 * slot);
-      if (++stage == L::STAGES) stage = 0, phase ^= 1u;
-      slot += 2;
-      if (slot >= A_SLOTS) slot -= A_SLOTS, a_phase ^= 1u;
+      if (lane == 0) mbar_arrive(written);
     }
-  } else {
+    if (!ok && lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
+  } else if (warp < L::SUM_WARPS) {
     // ---- sums ----
     const unsigned short* scale_row = static_cast<const unsigned short*>(p.scale) + static_cast<size_t>(min(n0 + row, p.N - 1)) * n_groups;
-    int set = 0;
-    uint32_t d_phase = 0;
+    const uint32_t sums = d0 + quarter + (warp / 4) * L::SUM_COLS;
     unsigned short next[GROUPS];
     auto load_scales = [&](int h) {
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) next[j] = __ldg(scale_row + min((2 * s0 + h) * GROUPS + j, n_groups - 1));
     };
 #pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i] = 0.0f;
+    for (int i = 0; i < L::SUM_COLS; ++i) acc[i] = 0.0f;
     if (halves > 0) load_scales(0);
+    if (lane == 0) {
+      for (int h = 0; h < SETS; ++h) mbar_arrive(ready + 8 * h);
+    }
+    int set = 0, slot = 0, freed = SETS % SLOTS;
+    uint32_t slot_phase = 0;
     for (int h = 0; h < halves; ++h) {
       float scale[GROUPS];
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) scale[j] = (2 * s0 + h) * GROUPS + j < n_groups ? Wide16<T>::value(next[j]) : 0.0f;
       if (h + 1 < halves) load_scales(h + 1);
-      if (!mbar_wait_warp(dfull + 8 * set, d_phase, abort_flag)) {
+      if (!mbar_wait_warp(done + 8 * slot, slot_phase, abort_flag)) {
         if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
         break;
       }
       tc_fence_after();
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
-        const uint32_t from = d0 + quarter + (set * GROUPS + j) * NT;
-        if constexpr (NT == 16) {
-          uint32_t r[16];
-          tmem_ld_x16(from, r);
-          tmem_ld_wait();
+        const uint32_t from = sums + (set * GROUPS + j) * NT;
+        uint32_t r[L::SUM_COLS];
+        if constexpr (L::SUM_COLS == 16) tmem_ld_x16(from, r);
+        else tmem_ld_x32(from, r);
+        tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[i] = fmaf(scale[j], __uint_as_float(r[i]), acc[i]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < NT; c += 32) {
-            uint32_t r[32];
-            tmem_ld_x32(from + c, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(scale[j], __uint_as_float(r[i]), acc[c + i]);
-          }
-        }
+        for (int i = 0; i < L::SUM_COLS; ++i) acc[i] = fmaf(scale[j], __uint_as_float(r[i]), acc[i]);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(dempty + 8 * set);
-      if (++set == L::SETS) set = 0, d_phase ^= 1u;
+      if (lane == 0) mbar_arrive(ready + 8 * freed);
+      if (++set == SETS) set = 0;
+      if (++freed == SLOTS) freed = 0;
+      if (++slot == SLOTS) slot = 0, slot_phase ^= 1u;
     }
   }
 
@@ -355,17 +355,18 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (p.epilogue != EPI_NONE) v = wide_activation(v + Wide16<T>::value(static_cast<const unsigned short*>(p.bias)[n]), p.epilogue);
     static_cast<T*>(p.c)[static_cast<size_t>(m) * p.N + n] = Wide16<T>::round(v);
   };
+  const int m0 = warp / 4 * L::SUM_COLS;  // first token of a warp of sums
   if (p.split == 1) {
-    if (warp < 4 && n0 + row < p.N) {
+    if (warp < L::SUM_WARPS && n0 + row < p.N) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        if (i < p.M) store(i, n0 + row, acc[i]);
+      for (int i = 0; i < L::SUM_COLS; ++i)
+        if (m0 + i < p.M) store(m0 + i, n0 + row, acc[i]);
     }
   } else {
     float* red = reinterpret_cast<float*>(smem + L::OFF_RED);
-    if (warp < 4) {
+    if (warp < L::SUM_WARPS) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) red[i * ROWS + row] = acc[i];
+      for (int i = 0; i < L::SUM_COLS; ++i) red[(m0 + i) * ROWS + row] = acc[i];
     }
     __syncwarp();
     cluster_sync_all();  // also after a failed wait: every wait is bounded
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 13) {
+  if (warp == L::MULTIPLY_WARP) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
@@ -428,7 +429,7 @@ int launch_wide(const void* a, const void* q, WideParams p, cudaStream_t s) {
   p.part = (stages + p.split - 1) / p.split;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles) * p.split);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(L::THREADS);
   cfg.dynamicSmemBytes = L::BYTES;
   cfg.stream = s;
   cudaLaunchAttribute attrs[2];
