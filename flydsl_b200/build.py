@@ -53,6 +53,7 @@ HEADERS = [
     "moe_pair_kernel.cuh",
     "mx_kernel.cuh",
     "mx_quant_kernel.cuh",
+    "w4.cuh",
     "launch.h",
     "decode_launch.h",
     "host_common.h",

@@ -3,27 +3,22 @@
 //
 //   c[m, n] = epilogue(sum_g scale[n, g] * sum_{k in g} (q[n, k] - z[n, g]) * a[m, k])
 //
-// Bound: the weight stream, N K / 2 bytes.  The multiply is the warp-level tensor instruction (16 weight rows x 8 tokens x 16
-// inputs, fp32 sums) on codes that stay in registers from the load to the multiply: a product of up to 64 tokens on
-// 4-bit codes has no operand that a shared-memory or tensor-memory instruction could take as it is.
-// A code becomes a 16-bit number, exactly, by putting it into the mantissa of 128 (bf16) or 64 (fp16); that constant and the zero
-// point leave again by way of the sum of the group's activations.  The scale multiplies the fp32 sum of its group, so no
-// weight is rounded.
+// Here: the entry, and products of up to 4 tokens as integers.  More tokens: flyb200_w4_wide.cu.
+// Bound: the weight stream, N K / 2 bytes; what is reached is 62 % of the copy rate (1 x 28672 x 8192 in 30.4 us, floor 18.5), and
+// what is left is instructions: three for 8 codes, and the joining of limbs and scales for every group.
 #include "../../include/flyb200.h"
 #include "host_common.h"
-#include "ptx.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "w4.cuh"
 
 #include <atomic>
-#include <cstdlib>
-#include <cstdio>
 
 using namespace flyb200;
 
 namespace {
 
+// Tokens of a pass: up to 4 as integers below, up to 64 in flyb200_w4_wide.cu.  us, integers / wide: 1 x 28672 x 8192 30.4 / 46,
+// 4 x 28672 x 8192 42.5 / 46.5, 8 x 28672 x 8192 58.5 / 46.5, 8 x 8192 x 8192 23.4 / 15.0.
+constexpr int FEW_TOKENS = 4, WIDE_TOKENS = 64;
 constexpr int WARPS = 16;
 constexpr int CHUNK = 128;  // inputs that a warp takes at a time: 64 bytes of a row of codes
 
@@ -42,32 +37,6 @@ struct W4Params {
   int batch;     // tiles between two meetings of the warps
   int red_at;    // bytes of shared memory ahead of the partial sums
 };
-
-template <typename T>
-struct Half;
-template <>
-struct Half<__nv_bfloat16> {
-  __device__ static float bits(uint32_t low) { return __uint_as_float(low << 16); }
-  __device__ static float value(__nv_bfloat16 v) { return __bfloat162float(v); }
-  __device__ static __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
-};
-template <>
-struct Half<__half> {
-  __device__ static float bits(uint32_t low) { return __half2float(__ushort_as_half(static_cast<unsigned short>(low))); }
-  __device__ static float value(__half v) { return __half2float(v); }
-  __device__ static __half round(float v) { return __float2half_rn(v); }
-};
-
-__device__ __forceinline__ float activation(float v, int epi) {
-  if (epi == FLYB200_EPI_BIAS_RELU) return fmaxf(v, 0.0f);
-  if (epi == FLYB200_EPI_BIAS_SILU) return v / (1.0f + expf(-v));
-  if (epi == FLYB200_EPI_BIAS_GELU) {  // the tanh form, as the other products'
-    const float y = 0.7978845608f * (v + 0.044715f * (v * v * v));
-    const float e = expf(-2.0f * fabsf(y));
-    return 0.5f * v * ((y > 0.0f ? 2.0f : 2.0f * e) / (1.0f + e));
-  }
-  return v;
-}
 
 // ---- asynchronous copies of 16 bytes, zeros where `in` is false ----
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
@@ -96,20 +65,20 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[WORDS]) {
   }
 }
 
-// ---- up to 8 tokens: integers ------------------------------------------------------------------------------------------------
+// ---- up to 4 tokens: integers ------------------------------------------------------------------------------------------------
 //
 // The codes are multiplied as they are, as bytes: a word of 8 codes becomes two registers of four (three instructions, where
 // 16-bit numbers take seven).  The activations of a group become integers of 23 bits, x = X 2^e with 2^e set by the largest
 // magnitude of the group, and an integer three signed bytes ("limbs"), X = l0 + 2^8 l1 + 2^16 l2, which the instruction takes as
-// three columns.  The products and their sums over a group are exact integers; what rounds is X, by 2^-23 of the group's largest
-// magnitude - as in an fp32 sum that holds it - and the fp32 sums over the groups.  An infinity or NaN makes its token NaN.
+// three columns.  The products and their sums over a group are exact integers; what rounds is X, by 2^-22 of the group's largest
+// magnitude - as much as an fp32 sum that holds it - and the fp32 sums over the groups.  An infinity or NaN makes its token NaN.
 //
-// Columns of an instruction: NT = 1, 2 (up to 2, 4 tokens): four for each token, the fourth unused; NT = 3 (up to 8 tokens):
-// instruction l takes limb l of eight tokens.
+// Columns of an instruction: four for each token, the fourth unused; NT = 1, 2 instructions for up to 2, 4 tokens.
 //
 // The accumulators start at the bits of 1.5 * 2^23, so that the sum D of a column comes out as the number 1.5 * 2^23 + D.
 // With its fp32 companions of a group, f = 2^e and f sum(X) of every limb, a column adds
-// scale * (f D - zero f sum(X)) to the result in fp32; the limbs are put together at the end.
+// scale * (f D - zero f sum(X)) to the result in fp32; the limbs are put together at the end.  f is kept as a quarter and the scale
+// as its fourfold, so that 1.5 * 2^23 f stays in range for the largest bf16 numbers.
 constexpr uint32_t INT_BITS = 0x4B400000u;
 constexpr float INT_BASE = 12582912.0f;
 
@@ -270,7 +239,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
     uint32_t top = 0u;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = Half<T>::bits(e & 1 ? in[e / 2] >> 16 : in[e / 2] & 0xFFFFu);
+      v[e] = W4<T>::value(e & 1 ? in[e / 2] >> 16 : in[e / 2] & 0xFFFFu);
       top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);  // by the bits: infinities and NaN above all others
     }
     const uint32_t lanes = 0xFFFFu << (lane & 16);
@@ -279,7 +248,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
     const bool finite = top < 0x7F800000u;
     const uint32_t e = max(top >> 23, 24u);                     // 2^(e - 127) <= max < 2^(e - 126)
     const float up = __uint_as_float((275u - e) << 23);         // 2^(148 - e): |v up| < 2^22
-    const float f = finite ? __uint_as_float((e - 21u) << 23) : __uint_as_float(0x7FFFFFFFu);
+    const float f = finite ? __uint_as_float((e - 23u) << 23) : __uint_as_float(0x7FFFFFFFu);
     uint32_t u[8];
     int sum[3] = {0, 0, 0};
 #pragma unroll
@@ -309,7 +278,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
   int col[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    col[t] = NT == 3 ? 3 * min(g, p.M - 1) + t : 3 * min(2 * t + (g >> 2), p.M - 1) + min(g & 3, 2);
+    col[t] = 3 * min(2 * t + (g >> 2), p.M - 1) + min(g & 3, 2);
     x_col[t] = smem_u32(xs) + col[t] * 128;
   }
   uint32_t x_chunk[NT][GROUPS * (G == 128 ? 2 : 1)];
@@ -317,10 +286,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < GROUPS * (G == 128 ? 2 : 1); ++i) x_chunk[t][i] = x_col[t] + chunk_place<G>(G == 128 ? 4 * c + 2 * i : (i * 4 + c) * WORDS, col[t]) * 8;
-  constexpr int TOKENS = NT == 3 ? 2 : NT;  // info of a lane: tokens 2 c, 2 c + 1, or 2 t + c / 2
-  const float4* info_at[TOKENS];
+  const float4* info_at[NT];  // of the tokens 2 t + c / 2
 #pragma unroll
-  for (int t = 0; t < TOKENS; ++t) info_at[t] = info + min(NT == 3 ? 2 * c + t : 2 * t + (c >> 1), p.M - 1);
+  for (int t = 0; t < NT; ++t) info_at[t] = info + min(2 * t + (c >> 1), p.M - 1);
   uint32_t w_chunk[GROUPS];
 #pragma unroll
   for (int j = 0; j < GROUPS; ++j) {
@@ -341,7 +309,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
       float scale[LOADS], zero[LOADS];
 #pragma unroll
       for (int u = 0; u < LOADS; ++u) {
-        scale[u] = Half<T>::bits(next_scale[u]);
+        scale[u] = 4.0f * W4<T>::value(next_scale[u]);
         zero[u] = -static_cast<float>(next_zero[u] & 15);
       }
       load_scales();
@@ -362,9 +330,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
             }
           }
         }
-        float4 about[TOKENS];
+        float4 about[NT];
 #pragma unroll
-        for (int t = 0; t < TOKENS; ++t) about[t] = info_at[t][info_first + j * p.M];
+        for (int t = 0; t < NT; ++t) about[t] = info_at[t][info_first + j * p.M];
 #pragma unroll
         for (int r = 0; r < MT; ++r) {
           uint32_t sum[NT][4];
@@ -389,8 +357,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
             for (int t = 0; t < NT; ++t)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const float4& a = about[NT == 3 ? e : t];
-                const float fx = NT == 3 ? (t == 0 ? a.x : t == 1 ? a.y : a.z) : c & 1 ? (e ? a.w : a.z) : (e ? a.y : a.x);
+                const float4& a = about[t];
+                const float fx = c & 1 ? (e ? a.w : a.z) : (e ? a.y : a.x);
                 acc[r][t][2 * h + e] = fmaf(s, fmaf(__uint_as_float(sum[t][2 * h + e]), a.w, fmaf(z, fx, -INT_BASE * a.w)), acc[r][t][2 * h + e]);
               }
           }
@@ -406,18 +374,12 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int n = 16 * r + 8 * h + g;
-        if constexpr (NT == 3) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (2 * c + e < p.M) part[(2 * c + e) * S::R + n] = fmaf(65536.0f, acc[r][2][2 * h + e], fmaf(256.0f, acc[r][1][2 * h + e], acc[r][0][2 * h + e]));
-        } else {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            float v = c & 1 ? 65536.0f * acc[r][t][2 * h] : fmaf(256.0f, acc[r][t][2 * h + 1], acc[r][t][2 * h]);
-            v += __shfl_xor_sync(0xffffffffu, v, 1);
-            const int m = 2 * t + (c >> 1);
-            if ((c & 1) == 0 && m < p.M) part[m * S::R + n] = v;
-          }
+        for (int t = 0; t < NT; ++t) {
+          float v = c & 1 ? 65536.0f * acc[r][t][2 * h] : fmaf(256.0f, acc[r][t][2 * h + 1], acc[r][t][2 * h]);
+          v += __shfl_xor_sync(0xffffffffu, v, 1);
+          const int m = 2 * t + (c >> 1);
+          if ((c & 1) == 0 && m < p.M) part[m * S::R + n] = v;
         }
       }
     if (++held < p.batch && tile + clusters < p.tiles) continue;
@@ -454,8 +416,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
         v = from[0];
         for (int w = 1; w < p.wk; ++w) v += from[w * p.M * S::R];
       }
-      if (p.epilogue != FLYB200_EPI_NONE) v = activation(v + Half<T>::value(static_cast<const T*>(p.bias)[row]), p.epilogue);
-      static_cast<T*>(p.c)[static_cast<size_t>(m) * p.N + row] = Half<T>::round(v);
+      if (p.epilogue != FLYB200_EPI_NONE) v = w4_activation(v + W4<T>::value(static_cast<const unsigned short*>(p.bias)[row]), p.epilogue);
+      static_cast<T*>(p.c)[static_cast<size_t>(m) * p.N + row] = W4<T>::round(v);
     }
     held = 0;
     __syncwarp();
@@ -497,7 +459,6 @@ cudaError_t clusters_at_once(Kernel kernel, int split, int sms, int smem, int* o
   cfg.numAttrs = 1;
   if (cudaError_t e = cudaOccupancyMaxActiveClusters(out, kernel, &cfg)) return e;
   if (*out < 1) *out = 1;
-  if (getenv("W4_SAY")) fprintf(stderr, "split %d clusters %d\n", split, *out);
   at.store(*out);
   return cudaSuccess;
 }
@@ -520,7 +481,6 @@ cudaError_t launch_int(W4Params p, int split, cudaStream_t s) {
   p.part = (steps + split - 1) / split;
   p.wk = 1;
   while (p.wk < WARPS && 2 * p.wk <= p.part) p.wk *= 2;
-  if (const char* e = getenv("W4_WK")) p.wk = atoi(e);
   const int tile_rows = WARPS / p.wk * S::R;
   p.tiles = (p.N + tile_rows - 1) / tile_rows;
   int clusters = 0;
@@ -558,8 +518,7 @@ template <typename T, int G, int MT, int NT>
 int split_of(const W4Params& p) {
   using S = IntShape<MT, NT>;
   const int steps = (p.K + CHUNK - 1) / CHUNK;
-  const char* e = getenv("W4_SPLITS");
-  for (int split = e ? atoi(e) : 1; split <= 8; split *= 2) {
+  for (int split = 1; split <= 8; split *= 2) {
     const int part = (steps + split - 1) / split;
     if (part * (split - 1) >= steps && split > 1) return 0;  // a block without a step
     if (S::RING + S::x_bytes(p.M, part, G) + S::red_bytes(p.M) <= S::SMEM) return split;
@@ -572,14 +531,10 @@ bool try_int(const W4Params& p, cudaStream_t s, cudaError_t& e) {
   if (split) e = launch_int<T, G, MT, NT>(p, split, s);
   return split != 0;
 }
-// Up to 8 tokens; false where they do not fit.
+// False where the activations of so many inputs do not fit.
 template <typename T, int G>
 bool few_tokens(const W4Params& p, cudaStream_t s, cudaError_t& e) {
-  const char* ev = getenv("W4_MT");
-  const int mt = ev ? atoi(ev) : 2;
-  if (mt == 1)
-    return p.M <= 2 ? try_int<T, G, 1, 1>(p, s, e) : p.M <= 4 ? try_int<T, G, 1, 2>(p, s, e) : try_int<T, G, 1, 3>(p, s, e);
-  return p.M <= 2 ? try_int<T, G, 2, 1>(p, s, e) : p.M <= 4 ? try_int<T, G, 2, 2>(p, s, e) : try_int<T, G, 1, 3>(p, s, e);
+  return p.M <= 2 ? try_int<T, G, 2, 1>(p, s, e) : try_int<T, G, 2, 2>(p, s, e);
 }
 template <typename T>
 bool few_tokens(const W4Params& p, int group, cudaStream_t s, cudaError_t& e) {
@@ -598,16 +553,15 @@ extern "C" int flyb200_gemv_w4a16(void* c, const void* a, const void* q, const v
   auto multiple = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
   if (!multiple(a, 16) || !multiple(q, 16) || !multiple(c, 2) || !multiple(scale, 2) || !multiple(bias, 2)) return FLYB200_E_BAD_ALIGN;
   if (M == 0) return FLYB200_OK;
-  const bool fp16 = dtype == FLYB200_DT_FP16, wide = K >= 256 && getenv("W4_WIDE") == nullptr;
-  const int block = wide && M > 8 ? 64 : 8;
-  for (int m = 0; m < M; m += block) {
-    const int tokens = M - m < block ? M - m : block;
+  const bool fp16 = dtype == FLYB200_DT_FP16;
+  for (int m = 0; m < M; m += WIDE_TOKENS) {
+    const int tokens = M - m < WIDE_TOKENS ? M - m : WIDE_TOKENS;
     char* cm = static_cast<char*>(c) + static_cast<size_t>(m) * N * 2;
     const char* am = static_cast<const char*>(a) + static_cast<size_t>(m) * K * 2;
     W4Params p = {cm, am, static_cast<const uint8_t*>(q), scale, static_cast<const uint8_t*>(zero), bias, tokens, N, K, epilogue};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
-    if (tokens <= 8 && getenv("W4_ALLWIDE") == nullptr && (fp16 ? few_tokens<__half>(p, group, s, e) : few_tokens<__nv_bfloat16>(p, group, s, e))) {
+    if (tokens <= FEW_TOKENS && (fp16 ? few_tokens<__half>(p, group, s, e) : few_tokens<__nv_bfloat16>(p, group, s, e))) {
       CUDA_TRY(e);
     } else {
       const int rc = host::gemv_w4_wide(cm, am, q, scale, zero, bias, tokens, N, K, group, fp16, epilogue, stream);

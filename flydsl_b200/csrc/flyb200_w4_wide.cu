@@ -1,4 +1,4 @@
-// libflyb200: products of 9 and more tokens on 4-bit weights (flyb200_gemv_w4a16) on the tensor core's own operand path.
+// libflyb200: products of 5 and more tokens on 4-bit weights (flyb200_gemv_w4a16) on the tensor core's own operand path.
 //
 //   c[m, n] = epilogue(sum_g scale[n, g] * sum_{k in g} (q[n, k] - z[n, g]) * a[m, k])
 //
@@ -8,14 +8,16 @@
 // group are read back from tensor memory and added to the result, times the row's scale, in registers: a thread is a row there too,
 // so neither scales nor zero points travel between threads, and no weight is rounded.
 //
-// Bound: decoding.  9 integer instructions (of 64 lanes a cycle and SM) and 4 of 16-bit arithmetic for 8 codes are 57 weights a cycle;
-// the weight stream at the copy rate is 46.
+// Bound: issue slots of the decoding.  13 instructions for 8 codes, 9 of them on the integer pipe (64 lanes a cycle and SM: 57 weights a
+// cycle, the stream at the copy rate is 46), and what moves, waits and sums around them: 16 x 18944 x 8192, where every SM has one
+// tile, takes 24.1 us (floor 12.2); 16 x 28672 x 8192, 1.5 tiles for an SM, 46.6.
+// Measured against it: the warp-level instruction on codes decoded in registers takes 57.5 us for 16 x 28672 x 8192, 154 for 32 tokens.
 #include "../../include/flyb200.h"
 #include "gemm_kernels.cuh"
 #include "host_common.h"
+#include "w4.cuh"
 
 #include <atomic>
-#include <cstdlib>
 #include <cstring>
 
 namespace flyb200 {
@@ -41,10 +43,11 @@ struct WideParams {
 
 template <int NT, int G>
 struct Wide {
-  // Warps: sums (a thread has a row and up to 32 tokens), one of loads, one of multiplies, two of nothing, groups of four that decode.
-  static constexpr int SUM_COLS = NT > 32 ? 32 : NT, SUM_WARPS = 4 * NT / SUM_COLS;
-  static constexpr int LOAD_WARP = SUM_WARPS, MULTIPLY_WARP = SUM_WARPS + 1, DECODE_WARP = SUM_WARPS + 4;
-  static constexpr int DECODERS = NT > 32 ? 3 : 4;
+  // Warps: sums (a thread has a row and up to 32 tokens; up to 32 tokens two sets, of the even and of the odd halves), one of loads,
+  // two of multiplies, one of nothing, groups of four that decode.
+  static constexpr int SUM_COLS = NT > 32 ? 32 : NT, SUM_WARPS = 8, SUM_SETS = NT > 32 ? 1 : 2;
+  static constexpr int LOAD_WARP = SUM_WARPS, MULTIPLY_WARP = SUM_WARPS + 1, MULTIPLIERS = 2, DECODE_WARP = SUM_WARPS + 4;
+  static constexpr int DECODERS = 3;
   static constexpr int THREADS = 32 * (DECODE_WARP + 4 * DECODERS);
   static constexpr int CODES = ROWS * 128, TOKENS = 4 * NT * 128;  // bytes of a stage
   static constexpr int STAGE = CODES + TOKENS;
@@ -56,42 +59,6 @@ struct Wide {
   static constexpr int SETS = FIT > SLOTS ? SLOTS : FIT;  // of sums of a half stage
   static_assert(SETS >= 1 && STAGES >= 3 && BYTES <= 227 * 1024, "shared and tensor memory");
 };
-
-template <typename T>
-struct Wide16;
-template <>
-struct Wide16<__nv_bfloat16> {
-  static constexpr uint32_t MAGIC = 0x4300u, FORMAT = 1;  // 128: the last place of its mantissa is 1
-  __device__ static uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  __device__ static float value(unsigned short v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
-  __device__ static __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
-};
-template <>
-struct Wide16<__half> {
-  static constexpr uint32_t MAGIC = 0x6400u, FORMAT = 0;  // 1024
-  __device__ static uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  __device__ static float value(unsigned short v) { return __half2float(__ushort_as_half(v)); }
-  __device__ static __half round(float v) { return __float2half_rn(v); }
-};
-
-// 8 codes of a word as four pairs of neighbours, less the zero point; `offset`: MAGIC + zero point, twice.
-template <typename T>
-__device__ __forceinline__ void decode_pairs(uint32_t w, uint32_t offset, uint32_t* d) {
-  const uint32_t odd = w >> 4;
-  constexpr uint32_t BITS = Wide16<T>::MAGIC * 0x10001u;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    uint32_t v = __byte_perm(w, odd, static_cast<uint32_t>(b) | static_cast<uint32_t>(4 + b) << 8), m;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(v), "r"(0x000F000Fu), "r"(BITS));  // (v & mask) | BITS
-    d[b] = Wide16<T>::sub(m, offset);
-  }
-}
 
 // Registers -> TMEM: 32 lanes x 32 consecutive 32-bit columns.
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -117,24 +84,20 @@ __device__ __forceinline__ void umma_ts_f16(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-__device__ __forceinline__ float wide_activation(float v, int epi) {
-  if (epi == EPI_BIAS_RELU) return fmaxf(v, 0.0f);
-  if (epi == EPI_BIAS_SILU) return v / (1.0f + expf(-v));
-  if (epi == EPI_BIAS_GELU) {
-    const float y = 0.7978845608f * (v + 0.044715f * (v * v * v));
-    const float e = expf(-2.0f * fabsf(y));
-    return 0.5f * v * ((y > 0.0f ? 2.0f : 2.0f * e) / (1.0f + e));
-  }
-  return v;
+// Up to 32 tokens most waits find their phase complete, above that few do (64 x 8192 x 28672, groups of 64: 61.3 us by looking first, 56.9).
+template <int NT>
+__device__ __forceinline__ bool wait_of(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return NT > 32 ? mbar_wait_warp(bar, parity, abort_flag) : mbar_wait_soon(bar, parity, abort_flag);
 }
 
 // Roles meet at barriers in shared memory, each wait of bounded length:
 //   full[stage]   codes and tokens of a stage have landed
-//   empty[stage]  multiplied (commit), so decoded too
-//   ready[slot]   half a stage of numbers is in tensor memory (4 warps), and the sums of the half SETS before it have left (SUM_WARPS)
+//   empty[stage]  multiplied (a commit for each half), so decoded too
+//   ready[slot]   half a stage of numbers is in tensor memory (4 warps), and the sums of the half SETS before it have left (4 warps, or 8)
 //   done[slot]    multiplied (commit): the sums are there, the numbers may go
-// The warp of multiplies sets the pace where it has more to do than this: a wait costs it about 120 cycles, a commit 100
-// (half a stage in 900 cycles with three of each, 540 with one and a half).
+// What set the pace, one after the other (us of 16 x 18944 x 8192): three waits and commits a half in one warp of multiplies (32.9),
+// two and a half (29.0), two such warps (24.1), and then
+// it is the decoding: a second set of sums, a third warp of multiplies, six slots, scales by way of shared memory change nothing.
 template <typename T, int G, int NT>
 __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     gemv_w4_wide_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_tokens, const WideParams p) {
@@ -153,10 +116,10 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::STAGES; ++s) {
       mbar_init(full + 8 * s, 1);
-      mbar_init(empty + 8 * s, 1);
+      mbar_init(empty + 8 * s, 2);
     }
     for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(ready + 8 * s, 4 + L::SUM_WARPS);
+      mbar_init(ready + 8 * s, 4 + L::SUM_WARPS / L::SUM_SETS);
       mbar_init(done + 8 * s, 1);
     }
     abort_flag[0] = 0;
@@ -194,7 +157,7 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     uint32_t phase = 0;
     bool ok = true;
     for (int s = s0; s < s1; ++s) {
-      if (!mbar_wait_warp(empty + 8 * stage, phase ^ 1u, abort_flag)) {
+      if (!wait_of<NT>(empty + 8 * stage, phase ^ 1u, abort_flag)) {
         report_failure(p.status, ST_TIMEOUT, abort_flag);
         ok = false;
         break;
@@ -218,31 +181,33 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
         mbar_wait(full + 8 * s, ph, abort_flag + 1);
       }
     }
-  } else if (warp == L::MULTIPLY_WARP) {
-    // ---- multiplies ----
+  } else if (warp >= L::MULTIPLY_WARP && warp < L::MULTIPLY_WARP + L::MULTIPLIERS) {
+    // ---- multiplies: of the first and of the second half of every stage ----
     const bool issuer = elect_one();
-    constexpr uint32_t idesc = umma_idesc(1, Wide16<T>::FORMAT, ROWS, NT);
-    int stage = 0, slot = 0, set = 0;
+    constexpr uint32_t idesc = umma_idesc(1, W4<T>::FORMAT, ROWS, NT);
+    const int mine = warp - L::MULTIPLY_WARP;
+    int stage = 0, slot = mine, set = mine % SETS;
     uint32_t phase = 0, slot_phase = 0;
-    for (int h = 0; h < halves; ++h) {
-      if (((h & 1) == 0 && !mbar_wait_warp(full + 8 * stage, phase, abort_flag)) || !mbar_wait_warp(ready + 8 * slot, slot_phase, abort_flag)) {
+    for (int h = mine; h < halves; h += 2) {
+      if (!wait_of<NT>(full + 8 * stage, phase, abort_flag) || !wait_of<NT>(ready + 8 * slot, slot_phase, abort_flag)) {
         report_failure(p.status, ST_TIMEOUT, abort_flag);
         break;
       }
       tc_fence_after();
       if (issuer) {
-        const uint32_t tokens = base + stage * L::STAGE + L::CODES + (h & 1) * 2 * NT * 128;
+        const uint32_t tokens = base + stage * L::STAGE + L::CODES + mine * 2 * NT * 128;
 #pragma unroll
         for (int k = 0; k < HALF_K / 16; ++k) {  // 16 inputs: 8 columns of numbers, 32 bytes of a token's 128
           const uint64_t bdesc = umma_desc_sw128_kmajor(tokens + (k / 4) * NT * 128) + static_cast<uint64_t>((k % 4) * 2);
           umma_ts_f16(d0 + (set * GROUPS + k * 16 / G) * NT, a0 + slot * HALF_COLS + k * 8, bdesc, idesc, k * 16 % G != 0 ? 1u : 0u);
         }
         umma_commit(done + 8 * slot);
-        if (h & 1) umma_commit(empty + 8 * stage);
+        umma_commit(empty + 8 * stage);
       }
-      if ((h & 1) && ++stage == L::STAGES) stage = 0, phase ^= 1u;
-      if (++slot == SLOTS) slot = 0, slot_phase ^= 1u;
-      if (++set == SETS) set = 0;
+      if (++stage == L::STAGES) stage = 0, phase ^= 1u;
+      slot += 2;
+      if (slot >= SLOTS) slot -= SLOTS, slot_phase ^= 1u;
+      set = (set + 2) % SETS;
     }
   } else if (warp >= L::DECODE_WARP) {
     // ---- decoding: group i takes the halves i, i + DECODERS, ...  The codes of the next one are read while the numbers of this one
@@ -260,7 +225,7 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     };
     uint4 w[4];
     auto read_codes = [&]() {
-      if (!mbar_wait_warp(full + 8 * stage, phase, abort_flag)) return false;
+      if (!wait_of<NT>(full + 8 * stage, phase, abort_flag)) return false;
       const uint32_t at = base + stage * L::STAGE + row * 128;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = ld_smem_v4(at + ((((h & 1) * 4 + i) ^ (row & 7)) << 4));
@@ -274,10 +239,10 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     while (h < halves && ok) {
       uint32_t offset[GROUPS];
 #pragma unroll
-      for (int j = 0; j < GROUPS; ++j) offset[j] = (Wide16<T>::MAGIC + (next[j] & 15u)) * 0x10001u;
+      for (int j = 0; j < GROUPS; ++j) offset[j] = (W4<T>::ZERO + (next[j] & 15u)) * 0x10001u;
       const int then = h + L::DECODERS;
       if (then < halves) load_zeros(then);
-      if (!(ok = mbar_wait_warp(done + 8 * slot, slot_phase ^ 1u, abort_flag))) break;
+      if (!(ok = wait_of<NT>(done + 8 * slot, slot_phase ^ 1u, abort_flag))) break;
       tc_fence_after();
       const uint32_t dst = a0 + quarter + slot * HALF_COLS;
 #pragma unroll
@@ -307,7 +272,8 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
   } else if (warp < L::SUM_WARPS) {
     // ---- sums ----
     const unsigned short* scale_row = static_cast<const unsigned short*>(p.scale) + static_cast<size_t>(min(n0 + row, p.N - 1)) * n_groups;
-    const uint32_t sums = d0 + quarter + (warp / 4) * L::SUM_COLS;
+    const int mine = L::SUM_SETS == 2 ? warp / 4 : 0;
+    const uint32_t sums = d0 + quarter + (L::SUM_SETS == 2 ? 0 : warp / 4) * L::SUM_COLS;
     unsigned short next[GROUPS];
     auto load_scales = [&](int h) {
 #pragma unroll
@@ -315,18 +281,18 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     };
 #pragma unroll
     for (int i = 0; i < L::SUM_COLS; ++i) acc[i] = 0.0f;
-    if (halves > 0) load_scales(0);
-    if (lane == 0) {
+    load_scales(mine);
+    if (lane == 0 && mine == 0) {
       for (int h = 0; h < SETS; ++h) mbar_arrive(ready + 8 * h);
     }
-    int set = 0, slot = 0, freed = SETS % SLOTS;
+    int set = mine % SETS, slot = mine, freed = (mine + SETS) % SLOTS;
     uint32_t slot_phase = 0;
-    for (int h = 0; h < halves; ++h) {
+    for (int h = mine; h < halves; h += L::SUM_SETS) {
       float scale[GROUPS];
 #pragma unroll
-      for (int j = 0; j < GROUPS; ++j) scale[j] = (2 * s0 + h) * GROUPS + j < n_groups ? Wide16<T>::value(next[j]) : 0.0f;
-      if (h + 1 < halves) load_scales(h + 1);
-      if (!mbar_wait_warp(done + 8 * slot, slot_phase, abort_flag)) {
+      for (int j = 0; j < GROUPS; ++j) scale[j] = (2 * s0 + h) * GROUPS + j < n_groups ? W4<T>::UNIT * W4<T>::value(next[j]) : 0.0f;
+      if (h + L::SUM_SETS < halves) load_scales(h + L::SUM_SETS);
+      if (!wait_of<NT>(done + 8 * slot, slot_phase, abort_flag)) {
         if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
         break;
       }
@@ -344,27 +310,40 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ready + 8 * freed);
-      if (++set == SETS) set = 0;
-      if (++freed == SLOTS) freed = 0;
-      if (++slot == SLOTS) slot = 0, slot_phase ^= 1u;
+      set = (set + L::SUM_SETS) % SETS, freed = (freed + L::SUM_SETS) % SLOTS;
+      slot += L::SUM_SETS;
+      if (slot >= SLOTS) slot -= SLOTS, slot_phase ^= 1u;
     }
   }
 
   // ---- the result: of a block by itself from registers, of a cluster through shared memory, added up in the order of its blocks ----
   auto store = [&](int m, int n, float v) {
-    if (p.epilogue != EPI_NONE) v = wide_activation(v + Wide16<T>::value(static_cast<const unsigned short*>(p.bias)[n]), p.epilogue);
-    static_cast<T*>(p.c)[static_cast<size_t>(m) * p.N + n] = Wide16<T>::round(v);
+    if (p.epilogue != EPI_NONE) v = w4_activation(v + W4<T>::value(static_cast<const unsigned short*>(p.bias)[n]), p.epilogue);
+    static_cast<T*>(p.c)[static_cast<size_t>(m) * p.N + n] = W4<T>::round(v);
   };
-  const int m0 = warp / 4 * L::SUM_COLS;  // first token of a warp of sums
+  const int m0 = L::SUM_SETS == 2 ? 0 : warp / 4 * L::SUM_COLS;  // first token of a warp of sums
+  float* red = reinterpret_cast<float*>(smem + L::OFF_RED);
+  int sum_warps = L::SUM_WARPS;
+  if constexpr (L::SUM_SETS == 2) {  // the odd halves' sums to the even ones'
+    if (warp >= 4 && warp < 8) {
+#pragma unroll
+      for (int i = 0; i < L::SUM_COLS; ++i) red[i * ROWS + row] = acc[i];
+    }
+    __syncthreads();
+    sum_warps = 4;
+    if (warp < 4) {
+#pragma unroll
+      for (int i = 0; i < L::SUM_COLS; ++i) acc[i] += red[i * ROWS + row];
+    }
+  }
   if (p.split == 1) {
-    if (warp < L::SUM_WARPS && n0 + row < p.N) {
+    if (warp < sum_warps && n0 + row < p.N) {
 #pragma unroll
       for (int i = 0; i < L::SUM_COLS; ++i)
         if (m0 + i < p.M) store(m0 + i, n0 + row, acc[i]);
     }
   } else {
-    float* red = reinterpret_cast<float*>(smem + L::OFF_RED);
-    if (warp < L::SUM_WARPS) {
+    if (warp < sum_warps) {
 #pragma unroll
       for (int i = 0; i < L::SUM_COLS; ++i) red[(m0 + i) * ROWS + row] = acc[i];
     }
@@ -425,7 +404,6 @@ int launch_wide(const void* a, const void* q, WideParams p, cudaStream_t s) {
   if (rc) return rc;
   const int tiles = (p.N + ROWS - 1) / ROWS, stages = (p.K + STAGE_K - 1) / STAGE_K;
   p.split = wide_split(tiles, stages);
-  if (const char* ev = getenv("W4_SPLITS")) p.split = atoi(ev);
   p.part = (stages + p.split - 1) / p.split;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles) * p.split);

@@ -40,7 +40,7 @@ int weight_image_map(CUtensorMap* m, const void* base, uint64_t n_rows, uint64_t
 // (FLYB200_MXFMT_*; 0 = E4M3, and for `fp4`).
 int gemm_mx_small(void* c, const void* a, const void* w, const void* sf_a, const void* sf_w, int M, int N, int K,
                   int outmode, bool fp4, void* stream, int a_format = 0, int w_format = 0);
-// flyb200_gemv_w4a16 on tcgen05.mma (flyb200_w4_wide.cu): up to 64 tokens, K of at least 256; arguments already checked.
+// flyb200_gemv_w4a16 on tcgen05.mma (flyb200_w4_wide.cu): up to 64 tokens; arguments already checked.
 int gemv_w4_wide(void* c, const void* a, const void* q, const void* scale, const void* zero, const void* bias, int M, int N, int K, int group,
                  bool fp16, int epilogue, void* stream);
 // Pointer to the current device's status word (first failed bounded wait wins).

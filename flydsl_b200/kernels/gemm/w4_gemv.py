@@ -11,11 +11,14 @@ The weights are read as they are stored: ``q`` uint8 [N, K / 2], two codes 0..15
 half (the packing of ``per_1x32_f4_quant``), ``s`` [N, K / group_size] in the type of the activations, ``z`` uint8
 [N, K / group_size] with zero points 0..15; without zero points the codes are signed numbers plus 8.  Group sizes 32, 64
 and 128.  ``epilogue``, ``bias`` [N] and ``stream`` are those of ``compile_preshuffle_gemm``; the output has the type of the
-activations.  Sums are fp32 and no weight is rounded on the way: code minus zero point is exact in 16 bits, and the scale
-multiplies the sum of its group.
+activations.  Sums are fp32 and no weight is rounded on the way: code minus zero point is exact, and the scale multiplies the
+sum of its group.  Up to 4 tokens the activations of a group are rounded to within 2^-22 of the group's largest magnitude (exact
+products and sums of integers); a token that holds an infinity or a NaN gives no finite number, and which of the two
+may depend on the number of tokens.
 
-Any number of tokens runs, in blocks of 32 that each stream the weights; from a few dozen tokens on the 8-bit products on the
-tensor core (``compile_preshuffle_gemm``) are the faster ones.
+Any number of tokens runs, in blocks of 64 that each stream the weights; for more than that the 8-bit products
+on the tensor core (``compile_preshuffle_gemm``) are the faster ones.  Weights, activations and scales are read in place, on
+the stream given; nothing is kept between calls, so a launch can be captured into a CUDA graph.
 """
 
 from __future__ import annotations

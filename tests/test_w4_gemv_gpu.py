@@ -2,9 +2,10 @@
 
 Tolerance: codes minus zero points and their products with 16-bit activations are exact; what rounds is the fp32 sums.  A term
 passes at most G / 16 tensor-core additions (each off by at most 2^-22 of the terms so far: its aligned sum keeps 24 bits and
-cuts), then the scale (K / (8 G) + 1 fused additions on a warp's way through its groups) and the sum over the warps (8) and
-splits (up to 16): c is off by at most (G / 16 * 4 + K / (8 G) + 26) 2^-24 of the sum of the magnitudes, plus half a step of
-its own type."""
+cuts), then the scale and the sum over the groups (K / G fused additions at most, in one chain), the sum of two such chains and
+over the blocks of a cluster (up to 8): c is off by at most (G / 16 * 4 + K / G + 10) 2^-24 of the sum of the magnitudes, plus half a
+step of its own type.  Up to 4 tokens the activations of a group are rounded to multiples of 2^-21 of the power of two at
+or below its largest magnitude, by half a multiple at most: the weights of the group times 2^-22 of that magnitude come on top."""
 
 import pytest
 import torch
@@ -44,7 +45,10 @@ def check(c, a, q, s, z, bias, group, epilogue="none"):
     c64, mag = a.double() @ w.t(), a.double().abs() @ w.abs().t()
     if epilogue != "none":
         c64, mag = c64 + bias.double(), mag + bias.double().abs()
-    sums = (group / 16 * 4 + k / (8 * group) + 26) * 2.0**-24 * mag
+    sums = (group / 16 * 4 + k / group + 10) * 2.0**-24 * mag
+    if len(a) <= 4:
+        top = a.double().abs().reshape(len(a), -1, group).amax(-1)
+        sums = sums + 2.0**-22 * top @ w.abs().reshape(len(w), -1, group).sum(-1).t()
     c64 = ACT[epilogue](c64)
     # relu, silu and gelu change a value by at most 1.13 of what its argument changes; exp and the quotients: 2^-20
     err, info = (c.double() - c64).abs(), torch.finfo(c.dtype)
@@ -128,6 +132,19 @@ def test_infinities_and_nan_stay_in_their_token():
     fn(c, a, q, s, z, None, 4, 100, torch.cuda.current_stream())
     assert bool(torch.isnan(c[1]).all()) and not bool(torch.isfinite(c[2]).any())
     check(c[[0, 3]], a[[0, 3]], q, s, z, None, 64)
+
+
+@pytest.mark.parametrize("m", [1, 4, 5, 40])
+def test_largest_and_smallest_activations(m):
+    """bf16 activations at both ends of its range; the weights bring the sums back into it."""
+    a, q, s, z, _ = make(m, 64, 256, 32, "bf16", True, 11)
+    fn = compile_w4a16_gemv(N=64, K=256, group_size=32, zero_points=True)
+    for size, scale in ((2.0**127, 2.0**-40), (2.0**-100, 2.0**60)):
+        x = (a.float().clamp(-1.9, 1.9) * size).to(torch.bfloat16)
+        t = torch.full_like(s, scale)
+        c = torch.empty(m, 64, dtype=torch.bfloat16, device="cuda")
+        fn(c, x, q, t, z, None, m, 64, torch.cuda.current_stream())
+        check(c, x, q, t, z, None, 32)
 
 
 def test_quantiser_and_product():
