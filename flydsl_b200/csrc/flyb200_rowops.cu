@@ -7,13 +7,15 @@
 // and of n or v, held in fp32: codes per row (scale s = max|v| * (1 / qmax), 0 -> 1; code = nearest(v / s), ties to even),
 // MXFP8 codes and E8M0 scales per 32 values as per_1x32_f8_quant, or values rounded to the type of x.
 //
-// Bound: memory.  Each input is read once and each output written once; a row stays in registers as raw 16-byte vectors
-// between its reductions and its conversion.
+// Bound: memory.  Each input is read once and each output written once; between its reductions and its conversion a row stays in
+// registers as the fp32 values that are converted.
 #include "../../include/flyb200.h"
 #include "host_common.h"
 #include "quant_kernel.cuh"
+#include "gemm_kernels.cuh"
 #include "mx_quant_kernel.cuh"
 
+#include <atomic>
 #include <cstring>
 
 using namespace flyb200;
@@ -34,6 +36,7 @@ struct RowParams {
   int warps_per_row;
   int w_f32;        // the weight is fp32, whatever x is
   float eps;
+  int* status;      // of bounded waits (wide gated rows)
 };
 
 template <typename T>
@@ -84,6 +87,24 @@ __device__ __forceinline__ Raw<T, N> pack(const float (&v)[N]) {
   for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(v[i]);
   return o;
 }
+// a + b, rounded once.  The sum of two 16-bit numbers in fp32 and then to 16 bits is the same: either fp32 holds it
+// exactly, or the smaller number is less than half a step of the larger one.
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> add_raw(const Raw<T, N>& a, const Raw<T, N>& b) {
+  Raw<T, N> o;
+  if constexpr (N == 8 && std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<__half2*>(&o)[i] = __hadd2(reinterpret_cast<const __half2*>(&a)[i], reinterpret_cast<const __half2*>(&b)[i]);
+  } else if constexpr (N == 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<__nv_bfloat162*>(&o)[i] = __hadd2(reinterpret_cast<const __nv_bfloat162*>(&a)[i], reinterpret_cast<const __nv_bfloat162*>(&b)[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(to_f32(a.v[i]) + to_f32(b.v[i]));
+  }
+  return o;
+}
 // The weights of N channels, of T or fp32.
 template <typename T, int N>
 __device__ __forceinline__ void load_weight(const RowParams& p, int k, float (&w)[N]) {
@@ -119,21 +140,23 @@ __device__ __forceinline__ float max_abs(float m, float v) {
 
 // Sum and maximum over the `wpr` warps of a row, the same in all of their threads.  `red`: 2 x 32 words of the block,
 // `first`: the row's first warp in the block, `bar`: a named barrier of the row's own.  Fixed order.
+template <bool SUM, bool MAX>
 __device__ __forceinline__ void row_reduce(float& sum, float& mx, int wpr, int first, int bar, float* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    mx = max_abs(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if constexpr (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if constexpr (MAX) mx = max_abs(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   if (wpr > 1) {
     if (lane == 0) red[warp] = sum, red[32 + warp] = mx;
     named_bar_sync(bar, 32 * wpr);
-    sum = lane < wpr ? red[first + lane] : 0.0f;
-    mx = lane < wpr ? red[32 + first + lane] : 0.0f;
+    if constexpr (SUM) sum = lane < wpr ? red[first + lane] : 0.0f;
+    if constexpr (MAX) mx = lane < wpr ? red[32 + first + lane] : 0.0f;
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      mx = max_abs(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if constexpr (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if constexpr (MAX) mx = max_abs(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     }
   }
 }
@@ -144,11 +167,18 @@ constexpr float QMAX_OF = Q == Q_INT8 ? 127.0f : 448.0f;
 // What turns the values of a row into codes: code = nearest(v * inv), or, where inv would leave the range of fp32, nearest(v / s).
 struct RowScale {
   float s;    // what is stored
-  float mul;  // qmax / max, of the values as they are passed to encode()
+  float mul;  // qmax / max, of the values as they are passed to encode(), and what its rounding left of it
+  float low;
   bool divide;
 };
+// Values in code units.  int8, where a step is as small against the largest values as against the smallest ones, has them rounded
+// once.
+template <int Q>
+__device__ __forceinline__ float in_units(float v, const RowScale& s) {
+  return Q == Q_INT8 ? fmaf(v, s.mul, v * s.low) : v * s.mul;
+}
 // Scale of a row whose values are `u * f` (f > 0) with max |u| = m: the code of u needs neither f nor s, u * (qmax / m) is the
-// same number with two roundings in all.
+// same number, rounded once or twice.
 template <int Q>
 __device__ __forceinline__ RowScale row_scale(float m, float f) {
   RowScale o;
@@ -156,6 +186,7 @@ __device__ __forceinline__ RowScale row_scale(float m, float f) {
   if (o.s == 0.0f) o.s = 1.0f;
   o.divide = false;
   o.mul = m > 0.0f ? __fdiv_rn(QMAX_OF<Q>, m) : 0.0f;
+  o.low = fmaf(-o.mul, m, m > 0.0f ? QMAX_OF<Q> : 0.0f) * (o.mul * (1.0f / QMAX_OF<Q>));
   return o;
 }
 // Whether the short form above holds: finite, and neither the maximum nor the scale near the lower end of fp32.
@@ -253,47 +284,41 @@ __global__ void __launch_bounds__(NV == 8 ? 512 : 1024) rmsnorm_row_kernel(RowPa
   const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + group;
   if (row >= p.rows) return;
   const T* xr = static_cast<const T*>(p.x) + row * p.x_stride;
-  Raw<T, N> raw[NV];
+  const T* rr = static_cast<const T*>(p.r) + row * p.r_stride;
+  T* hr = static_cast<T*>(p.h) + row * p.h_stride;
+  Raw<T, N> raw[NV], res[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int k = (i * tpr + tid) * N;
-    if (k < p.width) raw[i] = load_raw<T, N>(xr + k);
-    else memset(&raw[i], 0, sizeof(raw[i]));
-  }
-  if (p.r) {
-    const T* rr = static_cast<const T*>(p.r) + row * p.r_stride;
-    T* hr = static_cast<T*>(p.h) + row * p.h_stride;
-    Raw<T, N> res[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = (i * tpr + tid) * N;
-      if (k < p.width) res[i] = load_raw<T, N>(rr + k);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = (i * tpr + tid) * N;
-      if (k < p.width) {
-        float a[N], b[N];
-        unpack(raw[i], a);
-        unpack(res[i], b);
-#pragma unroll
-        for (int j = 0; j < N; ++j) a[j] += b[j];
-        raw[i] = pack<T, N>(a);
-        store_raw<T, N>(hr + k, raw[i]);
-      }
+    if (k < p.width) {
+      raw[i] = load_raw<T, N>(xr + k);
+      if (p.r) res[i] = load_raw<T, N>(rr + k);
     }
   }
-  float sum = 0.0f, mx = 0.0f;
+  float v[NV][N], sum = 0.0f, mx = 0.0f;  // v: h w
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int k = (i * tpr + tid) * N;
-    if (k >= p.width) break;
-    float h[N], w[N];
-    unpack(raw[i], h);
-    if constexpr (ROWQ) load_weight<T, N>(p, k, w);
-    norm_stats<ROWQ, N>(h, w, sum, mx);
+    if (k >= p.width) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i][j] = 0.0f;
+      continue;
+    }
+    if (p.r) {
+      raw[i] = add_raw<T, N>(raw[i], res[i]);
+      store_raw<T, N>(hr + k, raw[i]);
+    }
+    float w[N];
+    unpack(raw[i], v[i]);
+    load_weight<T, N>(p, k, w);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      sum = fmaf(v[i][j], v[i][j], sum);
+      v[i][j] *= w[j];
+      if constexpr (ROWQ) mx = max_abs(mx, v[i][j]);
+    }
   }
-  row_reduce(sum, mx, wpr, group * wpr, 1 + group, red);
+  row_reduce<true, ROWQ>(sum, mx, wpr, group * wpr, 1 + group, red);
   const float f = __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(p.width)), p.eps));
 
   if constexpr (ROWQ) {
@@ -306,27 +331,23 @@ __global__ void __launch_bounds__(NV == 8 ? 512 : 1024) rmsnorm_row_kernel(RowPa
       for (int i = 0; i < NV; ++i) {
         const int k = (i * tpr + tid) * N;
         if (k >= p.width) break;
-        float h[N], w[N];
-        unpack(raw[i], h);
-        load_weight<T, N>(p, k, w);
 #pragma unroll
-        for (int j = 0; j < N; ++j) h[j] = h[j] * w[j] * s.mul;
-        store_codes<Q, N>(yr + k, h);
+        for (int j = 0; j < N; ++j) v[i][j] = in_units<Q>(v[i][j], s);
+        store_codes<Q, N>(yr + k, v[i]);
       }
     } else {  // the same branch in all threads of the row
       float amax = 0.0f, none = 0.0f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int k = (i * tpr + tid) * N;
-        if (k >= p.width) break;
-        float h[N], w[N];
-        unpack(raw[i], h);
-        load_weight<T, N>(p, k, w);
+        if ((i * tpr + tid) * N >= p.width) break;
 #pragma unroll
-        for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(scrub(h[j] * w[j] * f, QMAX_OF<Q>)));
+        for (int j = 0; j < N; ++j) {
+          v[i][j] *= f;
+          amax = fmaxf(amax, fabsf(scrub(v[i][j], QMAX_OF<Q>)));
+        }
       }
       if (wpr > 1) named_bar_sync(1 + group, tpr);  // `red` is read above
-      row_reduce(none, amax, wpr, group * wpr, 1 + group, red);
+      row_reduce<false, true>(none, amax, wpr, group * wpr, 1 + group, red);
       float s = __fmul_rn(amax, 1.0f / QMAX_OF<Q>);
       if (s == 0.0f) s = 1.0f;
       if (tid == 0) *scale = s;
@@ -334,12 +355,7 @@ __global__ void __launch_bounds__(NV == 8 ? 512 : 1024) rmsnorm_row_kernel(RowPa
       for (int i = 0; i < NV; ++i) {
         const int k = (i * tpr + tid) * N;
         if (k >= p.width) break;
-        float h[N], w[N];
-        unpack(raw[i], h);
-        load_weight<T, N>(p, k, w);
-#pragma unroll
-        for (int j = 0; j < N; ++j) h[j] = h[j] * w[j] * f;
-        store_codes_divided<Q, N>(yr + k, h, s);
+        store_codes_divided<Q, N>(yr + k, v[i], s);
       }
     }
   } else {
@@ -347,17 +363,12 @@ __global__ void __launch_bounds__(NV == 8 ? 512 : 1024) rmsnorm_row_kernel(RowPa
     for (int i = 0; i < NV; ++i) {
       const int k = (i * tpr + tid) * N;
       const bool in = k < p.width;
-      float h[N] = {}, w[N];
-      if (in) {
-        unpack(raw[i], h);
-        load_weight<T, N>(p, k, w);
 #pragma unroll
-        for (int j = 0; j < N; ++j) h[j] = h[j] * w[j] * f;
-      }
+      for (int j = 0; j < N; ++j) v[i][j] *= f;
       if constexpr (Q == Q_MXFP8) {
-        store_mx<N>(static_cast<uint8_t*>(p.y) + row * p.width, static_cast<uint8_t*>(p.scale) + row * (p.width / 32), k, in, h);
+        store_mx<N>(static_cast<uint8_t*>(p.y) + row * p.width, static_cast<uint8_t*>(p.scale) + row * (p.width / 32), k, in, v[i]);
       } else if (in) {
-        store_raw<T, N>(static_cast<T*>(p.y) + row * p.width + k, pack<T, N>(h));
+        store_raw<T, N>(static_cast<T*>(p.y) + row * p.width + k, pack<T, N>(v[i]));
       }
     }
   }
@@ -394,10 +405,10 @@ __global__ void __launch_bounds__(512) rmsnorm_any_kernel(RowParams p) {
       if constexpr (ROWQ) load_weight<T, N>(p, k, w);
       norm_stats<ROWQ, N>(h, w, sum, mx);
     }
-    row_reduce(sum, mx, wpr, 0, 1, red);
+    row_reduce<true, ROWQ>(sum, mx, wpr, 0, 1, red);
     __syncthreads();  // `red` is used again
     const float f = __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(p.width)), p.eps));
-    RowScale s = {1.0f, 0.0f, false};
+    RowScale s = {1.0f, 0.0f, 0.0f, false};
     if constexpr (ROWQ) {
       if (row_is_plain<Q>(mx, f)) {
         s = row_scale<Q>(mx, f);
@@ -410,7 +421,7 @@ __global__ void __launch_bounds__(512) rmsnorm_any_kernel(RowParams p) {
 #pragma unroll
           for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(scrub(h[j] * w[j] * f, QMAX_OF<Q>)));
         }
-        row_reduce(none, amax, wpr, 0, 1, red);
+        row_reduce<false, true>(none, amax, wpr, 0, 1, red);
         __syncthreads();
         s.s = __fmul_rn(amax, 1.0f / QMAX_OF<Q>);
         if (s.s == 0.0f) s.s = 1.0f;
@@ -426,7 +437,7 @@ __global__ void __launch_bounds__(512) rmsnorm_any_kernel(RowParams p) {
         unpack(load_raw<T, N>(xr + k), h);
         load_weight<T, N>(p, k, w);
 #pragma unroll
-        for (int j = 0; j < N; ++j) h[j] = h[j] * w[j] * (ROWQ && !s.divide ? s.mul : f);
+        for (int j = 0; j < N; ++j) h[j] = ROWQ && !s.divide ? in_units<Q>(h[j] * w[j], s) : h[j] * w[j] * f;
       }
       if constexpr (ROWQ) {
         uint8_t* y = static_cast<uint8_t*>(p.y) + row * p.width + k;
@@ -442,8 +453,19 @@ __global__ void __launch_bounds__(512) rmsnorm_any_kernel(RowParams p) {
 
 // ---- gated activation ---------------------------------------------------------------------------------------------------
 
-// g / (1 + exp(-g)) * u.  1 + exp(-g) is infinite below g = -88: the quotient is then the zero that silu tends to.
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
+// g / (1 + exp(-g)) * u.  exp(-g) = 2^t (1 + ln 2 lo) with t + lo = -g log2(e), lo what the rounding of t left; then g times the reciprocal,
+// which one step of Newton's method makes good to its last place.  From 1 + exp(-g) = 2^126 on (g < -87) the reciprocal is 0, as
+// the value that silu tends to.  Beyond +-88 neither the sum nor the reciprocal changes; the exponent stays there, where 2^t is
+// finite.  NaN comes back with the factor g, and -Inf times 0 is NaN.
+__device__ __forceinline__ float gated(float g, float u) {
+  const float x = fmaxf(fminf(g, 88.0f), -88.0f), t = x * -1.44269504f, lo = fmaf(x, -1.44269504f, -t);
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  const float d = 1.0f + fmaf(e, lo * 0.693147181f, e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  if (d < 8.5e37f) r = fmaf(fmaf(-d, r, 1.0f), r, r);
+  return g * r * u;
+}
 
 template <typename T, int N>
 __device__ __forceinline__ void gated_at(const T* xr, int width, int k, float (&v)[N]) {
@@ -488,7 +510,7 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
       mx = max_abs(mx, v[i][j]);
     }
   }
-  row_reduce(none, mx, wpr, group * wpr, 1 + group, red);
+  row_reduce<false, true>(none, mx, wpr, group * wpr, 1 + group, red);
   uint8_t* yr = static_cast<uint8_t*>(p.y) + row * p.width;
   float* scale = static_cast<float*>(p.scale) + row;
   if (row_is_plain<Q>(mx, 1.0f)) {
@@ -499,7 +521,7 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
       const int k = (i * tpr + tid) * N;
       if (k >= p.width) break;
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[i][j] *= s.mul;
+      for (int j = 0; j < N; ++j) v[i][j] = in_units<Q>(v[i][j], s);
       store_codes<Q, N>(yr + k, v[i]);
     }
   } else {
@@ -511,7 +533,7 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
       for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(scrub(v[i][j], QMAX_OF<Q>)));
     }
     if (wpr > 1) named_bar_sync(1 + group, tpr);  // `red` is read above
-    row_reduce(none, amax, wpr, group * wpr, 1 + group, red);
+    row_reduce<false, true>(none, amax, wpr, group * wpr, 1 + group, red);
     float s = __fmul_rn(amax, 1.0f / QMAX_OF<Q>);
     if (s == 0.0f) s = 1.0f;
     if (tid == 0) *scale = s;
@@ -520,6 +542,133 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
       const int k = (i * tpr + tid) * N;
       if (k >= p.width) break;
       store_codes_divided<Q, N>(yr + k, v[i], s);
+    }
+  }
+}
+
+// Per-row scale of wide rows, many of them: a row in registers is more than half of an SM's, so there is no second block whose loads
+// could go on while this one reduces, converts and stores.  Here a warp of its own brings the rows, chunk by chunk and over
+// their ends, into a ring in shared memory by bulk copies; the others take a vector of every chunk per thread.
+// us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, RING_TIME here (floor 180).
+constexpr int RING_WARPS = 16, RING_THREADS = 32 * RING_WARPS;
+constexpr int RING_CHUNK = 16 * RING_THREADS;                   // bytes of gate values, and as many of up values
+constexpr int RING_SLOTS = 13;
+constexpr int RING_BYTES = RING_SLOTS * 2 * RING_CHUNK + 512;
+
+template <typename T, int Q, int NV>
+__global__ void __launch_bounds__(RING_THREADS + 32, 1) silu_ring_kernel(RowParams p) {
+  constexpr int N = VEC_OF<T>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float reds[3][64];  // of even rows, of odd rows, of the second maximum
+  const int warp = warp_index(), lane = threadIdx.x & 31, tid = threadIdx.x;
+  const uint32_t base = smem_u32(smem), full = base + RING_SLOTS * 2 * RING_CHUNK + 16, empty = full + 8 * RING_SLOTS;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + RING_SLOTS * 2 * RING_CHUNK);
+  if (tid == 0) {
+    for (int i = 0; i < RING_SLOTS; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, RING_WARPS);
+    }
+    abort_flag[0] = 0;
+    abort_flag[1] = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait(p.x, p.y, p.scale);
+  pdl_trigger();
+  int slot = 0;
+  uint32_t phase = 0;
+  if (warp == RING_WARPS) {
+    const bool issuer = elect_one();
+    const uint64_t once = l2_policy_evict_first();
+    int issued = 0;
+    bool ok = true;
+    for (long long row = blockIdx.x; row < p.rows && ok; row += gridDim.x) {
+      const T* xr = static_cast<const T*>(p.x) + row * p.x_stride;
+      for (int k = 0; k < p.width; k += RING_THREADS * N) {
+        if (!mbar_wait_warp(empty + 8 * slot, phase ^ 1u, abort_flag)) {
+          report_failure(p.status, ST_TIMEOUT, abort_flag);
+          ok = false;
+          break;
+        }
+        if (issuer) {
+          const uint32_t bytes = min(RING_THREADS * N, p.width - k) * static_cast<int>(sizeof(T)), at = base + slot * 2 * RING_CHUNK;
+          mbar_expect_tx(full + 8 * slot, 2 * bytes);
+          bulk_load_1d(at, xr + k, bytes, full + 8 * slot, once);
+          bulk_load_1d(at + RING_CHUNK, xr + p.width + k, bytes, full + 8 * slot, once);
+        }
+        ++issued;
+        if (++slot == RING_SLOTS) slot = 0, phase ^= 1u;
+      }
+    }
+    if (!ok || *abort_flag) {  // copies in flight land before the block leaves
+      const int pending = min(issued, RING_SLOTS);
+      for (int i = 0; i < pending; ++i) {
+        int s = slot - 1 - i;
+        uint32_t ph = phase;
+        if (s < 0) s += RING_SLOTS, ph ^= 1u;
+        mbar_wait(full + 8 * s, ph, abort_flag + 1);
+      }
+    }
+    return;
+  }
+  bool ok = true;  // a warp that gave up goes on through the barriers without waiting
+  int odd = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    float v[NV][N], mx = 0.0f, none = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (ok && !mbar_wait_warp(full + 8 * slot, phase, abort_flag)) {
+        if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
+        ok = false;
+      }
+      if ((i * RING_THREADS + tid) * N < p.width) {
+        float u[N];
+        const uint8_t* at = smem + slot * 2 * RING_CHUNK + tid * 16;
+        unpack(load_raw<T, N>(reinterpret_cast<const T*>(at)), v[i]);
+        unpack(load_raw<T, N>(reinterpret_cast<const T*>(at + RING_CHUNK)), u);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          v[i][j] = gated(v[i][j], u[j]);
+          mx = max_abs(mx, v[i][j]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + 8 * slot);
+      if (++slot == RING_SLOTS) slot = 0, phase ^= 1u;
+    }
+    row_reduce<false, true>(none, mx, RING_WARPS, 0, 1, reds[odd]);  // nobody writes over it before all are at the next row's barrier
+    odd ^= 1;
+    uint8_t* yr = static_cast<uint8_t*>(p.y) + row * p.width;
+    float* scale = static_cast<float*>(p.scale) + row;
+    if (row_is_plain<Q>(mx, 1.0f)) {
+      const RowScale s = row_scale<Q>(mx, 1.0f);
+      if (tid == 0) *scale = s.s;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int k = (i * RING_THREADS + tid) * N;
+        if (k >= p.width) break;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i][j] = in_units<Q>(v[i][j], s);
+        store_codes<Q, N>(yr + k, v[i]);
+      }
+    } else {
+      float amax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if ((i * RING_THREADS + tid) * N >= p.width) break;
+#pragma unroll
+        for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(scrub(v[i][j], QMAX_OF<Q>)));
+      }
+      row_reduce<false, true>(none, amax, RING_WARPS, 0, 1, reds[2]);
+      float s = __fmul_rn(amax, 1.0f / QMAX_OF<Q>);
+      if (s == 0.0f) s = 1.0f;
+      if (tid == 0) *scale = s;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int k = (i * RING_THREADS + tid) * N;
+        if (k >= p.width) break;
+        store_codes_divided<Q, N>(yr + k, v[i], s);
+      }
     }
   }
 }
@@ -539,9 +688,9 @@ __global__ void __launch_bounds__(512) silu_any_kernel(RowParams p) {
 #pragma unroll
       for (int j = 0; j < N; ++j) mx = max_abs(mx, v[j]);
     }
-    row_reduce(none, mx, wpr, 0, 1, red);
+    row_reduce<false, true>(none, mx, wpr, 0, 1, red);
     __syncthreads();
-    RowScale s = {1.0f, 0.0f, false};
+    RowScale s = {1.0f, 0.0f, 0.0f, false};
     if (row_is_plain<Q>(mx, 1.0f)) {
       s = row_scale<Q>(mx, 1.0f);
     } else {
@@ -551,7 +700,7 @@ __global__ void __launch_bounds__(512) silu_any_kernel(RowParams p) {
 #pragma unroll
         for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(scrub(v[j], QMAX_OF<Q>)));
       }
-      row_reduce(none, amax, wpr, 0, 1, red);
+      row_reduce<false, true>(none, amax, wpr, 0, 1, red);
       __syncthreads();
       s.s = __fmul_rn(amax, 1.0f / QMAX_OF<Q>);
       if (s.s == 0.0f) s.s = 1.0f;
@@ -565,7 +714,7 @@ __global__ void __launch_bounds__(512) silu_any_kernel(RowParams p) {
         store_codes_divided<Q, N>(yr + k, v, s.s);
       } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] *= s.mul;
+        for (int j = 0; j < N; ++j) v[j] = in_units<Q>(v[j], s);
         store_codes<Q, N>(yr + k, v);
       }
     }
@@ -621,7 +770,8 @@ template <typename T, int Q>
 cudaError_t launch_norm(RowParams p, bool vectors, cudaStream_t s) {
   constexpr int N = VEC_OF<T>;
   const int vecs = p.width / N;
-  int wpr = vectors ? warps_per_row(p.rows, vecs, 4, 32) : 0, nv = 0;
+  int wpr = vectors ? warps_per_row(p.rows, vecs, N == 8 ? 2 : 4, 32) : 0, nv = 0;
+  if (vectors && !wpr) wpr = warps_per_row(p.rows, vecs, 4, 32);
   if (wpr) nv = (vecs + 32 * wpr - 1) / (32 * wpr);
   else if (vectors && (wpr = warps_per_row(p.rows, vecs, 8, 16)) != 0) nv = 8;
   if (!nv) {
@@ -638,6 +788,25 @@ cudaError_t launch_norm(RowParams p, bool vectors, cudaStream_t s) {
                    : host::launch_dependent(rmsnorm_row_kernel<T, Q, 8>, grid, t, 0, s, p);
 }
 
+// Vectors of a row from which on the ring is taken.
+constexpr int RING_FROM = 2 * RING_THREADS;
+
+template <typename T, int Q, int NV>
+cudaError_t launch_silu_ring(RowParams p, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load(std::memory_order_acquire) & bit)) {
+    if (cudaError_t e = cudaFuncSetAttribute(silu_ring_kernel<T, Q, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES)) return e;
+    done.fetch_or(bit, std::memory_order_release);
+  }
+  if (host::status_word(&p.status)) return cudaErrorInvalidDevice;
+  int sms = 0;
+  if (host::sm_count(&sms)) return cudaErrorInvalidDevice;
+  return host::launch_dependent(silu_ring_kernel<T, Q, NV>, dim3(p.rows < sms ? p.rows : sms), RING_THREADS + 32, RING_BYTES, s, p);
+}
+
 template <typename T, int Q>
 cudaError_t launch_silu(RowParams p, bool vectors, cudaStream_t s) {
   constexpr int N = VEC_OF<T>;
@@ -649,6 +818,15 @@ cudaError_t launch_silu(RowParams p, bool vectors, cudaStream_t s) {
                    : host::launch_dependent(silu_flat_kernel<T, Q, 1>, dim3(static_cast<unsigned>(blocks)), 256, 0, s, p);
   } else {
     const int vecs = p.width / N;
+    if (vectors && vecs > RING_FROM && vecs <= 8 * RING_THREADS && p.rows > 148) {
+      const int nv = (vecs + RING_THREADS - 1) / RING_THREADS;
+      return nv <= 3   ? launch_silu_ring<T, Q, 3>(p, s)
+             : nv == 4 ? launch_silu_ring<T, Q, 4>(p, s)
+             : nv == 5 ? launch_silu_ring<T, Q, 5>(p, s)
+             : nv == 6 ? launch_silu_ring<T, Q, 6>(p, s)
+             : nv == 7 ? launch_silu_ring<T, Q, 7>(p, s)
+                       : launch_silu_ring<T, Q, 8>(p, s);
+    }
     const int wpr = vectors ? warps_per_row(p.rows, vecs, 4, 32) : 0;
     if (!wpr) {
       const dim3 grid(p.rows < ANY_BLOCKS ? p.rows : ANY_BLOCKS);
@@ -701,7 +879,7 @@ int flyb200_rmsnorm_quant(void* y, void* scale, void* residual_out, const void* 
   bool vectors = K % n == 0 && x_stride % n == 0 && multiple(x, 16) && multiple(weight, 16) && multiple(y, quant == Q_NONE ? 16 : n);
   if (residual)
     vectors = vectors && residual_stride % n == 0 && residual_out_stride % n == 0 && multiple(residual, 16) && multiple(residual_out, 16);
-  const RowParams p = {y, scale, residual_out, x, residual, weight, x_stride, residual_stride, residual_out_stride, rows, K, 0, weight_f32 ? 1 : 0, eps};
+  const RowParams p = {y, scale, residual_out, x, residual, weight, x_stride, residual_stride, residual_out_stride, rows, K, 0, weight_f32 ? 1 : 0, eps, nullptr};
   CUDA_TRY(launch_rows<true>(p, x_dtype, quant, vectors, static_cast<cudaStream_t>(stream)));
   return FLYB200_OK;
 }
@@ -715,7 +893,7 @@ int flyb200_silu_mul_quant(void* y, void* scale, const void* x, int rows, int in
   if (!multiple(x, e) || !multiple(y, quant == Q_NONE ? e : 1) || (quant != Q_MXFP8 && !multiple(scale, 4))) return FLYB200_E_BAD_ALIGN;
   if (rows == 0) return FLYB200_OK;
   const bool vectors = inter % n == 0 && x_stride % n == 0 && multiple(x, 16) && multiple(y, quant == Q_NONE ? 16 : n);
-  const RowParams p = {y, scale, nullptr, x, nullptr, nullptr, x_stride, 0, 0, rows, inter, 0, 0, 0.0f};
+  const RowParams p = {y, scale, nullptr, x, nullptr, nullptr, x_stride, 0, 0, rows, inter, 0, 0, 0.0f, nullptr};
   if (quant == Q_NONE || quant == Q_MXFP8) {
     const long long blocks = ((vectors ? inter / n : inter) + 255ll) / 256 * rows;
     if (blocks > 0x7fffffffll) return FLYB200_E_UNSUPPORTED;

@@ -43,11 +43,10 @@ struct WideParams {
 
 template <int NT, int G>
 struct Wide {
-  // Warps: sums (a thread has a row and up to 32 tokens; up to 32 tokens two sets, of the even and of the odd halves), one of loads,
-  // two of multiplies, one of nothing, groups of four that decode.
-  static constexpr int SUM_COLS = NT > 32 ? 32 : NT, SUM_WARPS = 8, SUM_SETS = NT > 32 ? 1 : 2;
+  // Warps: sums (a thread has a row and up to 32 tokens), one of loads, two of multiplies, one of nothing, groups of four that decode.
+  static constexpr int SUM_COLS = NT > 32 ? 32 : NT, SUM_WARPS = 4 * NT / SUM_COLS;
   static constexpr int LOAD_WARP = SUM_WARPS, MULTIPLY_WARP = SUM_WARPS + 1, MULTIPLIERS = 2, DECODE_WARP = SUM_WARPS + 4;
-  static constexpr int DECODERS = 3;
+  static constexpr int DECODERS = NT > 32 ? 2 : 4;  // 2: what the registers of the sums leave
   static constexpr int THREADS = 32 * (DECODE_WARP + 4 * DECODERS);
   static constexpr int CODES = ROWS * 128, TOKENS = 4 * NT * 128;  // bytes of a stage
   static constexpr int STAGE = CODES + TOKENS;
@@ -58,6 +57,11 @@ struct Wide {
   static constexpr int FIT = (static_cast<int>(TMEM_COLS) - SLOTS * HALF_COLS) / (GROUPS * NT);
   static constexpr int SETS = FIT > SLOTS ? SLOTS : FIT;  // of sums of a half stage
   static_assert(SETS >= 1 && STAGES >= 3 && BYTES <= 227 * 1024, "shared and tensor memory");
+  // A wait by parity is only sound where the phase before the awaited one is known to be complete.  The two multiplying warps take the
+  // even and the odd halves, each at its own pace: a group that came to half h by way of halves of the other kind (three
+  // groups) could wait for half h - SLOTS before h - 2 SLOTS is multiplied, and be let through.  With two or four groups a slot is always
+  // written by the same one.
+  static_assert(SLOTS % DECODERS == 0 && SLOTS % MULTIPLIERS == 0, "a slot's waits follow each other in one warp");
 };
 
 // Registers -> TMEM: 32 lanes x 32 consecutive 32-bit columns.
@@ -119,7 +123,7 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
       mbar_init(empty + 8 * s, 2);
     }
     for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(ready + 8 * s, 4 + L::SUM_WARPS / L::SUM_SETS);
+      mbar_init(ready + 8 * s, 4 + L::SUM_WARPS);
       mbar_init(done + 8 * s, 1);
     }
     abort_flag[0] = 0;
@@ -272,8 +276,7 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
   } else if (warp < L::SUM_WARPS) {
     // ---- sums ----
     const unsigned short* scale_row = static_cast<const unsigned short*>(p.scale) + static_cast<size_t>(min(n0 + row, p.N - 1)) * n_groups;
-    const int mine = L::SUM_SETS == 2 ? warp / 4 : 0;
-    const uint32_t sums = d0 + quarter + (L::SUM_SETS == 2 ? 0 : warp / 4) * L::SUM_COLS;
+    const uint32_t sums = d0 + quarter + (warp / 4) * L::SUM_COLS;
     unsigned short next[GROUPS];
     auto load_scales = [&](int h) {
 #pragma unroll
@@ -281,17 +284,17 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     };
 #pragma unroll
     for (int i = 0; i < L::SUM_COLS; ++i) acc[i] = 0.0f;
-    load_scales(mine);
-    if (lane == 0 && mine == 0) {
+    load_scales(0);
+    if (lane == 0) {
       for (int h = 0; h < SETS; ++h) mbar_arrive(ready + 8 * h);
     }
-    int set = mine % SETS, slot = mine, freed = (mine + SETS) % SLOTS;
+    int set = 0, slot = 0, freed = SETS % SLOTS;
     uint32_t slot_phase = 0;
-    for (int h = mine; h < halves; h += L::SUM_SETS) {
+    for (int h = 0; h < halves; ++h) {
       float scale[GROUPS];
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) scale[j] = (2 * s0 + h) * GROUPS + j < n_groups ? W4<T>::UNIT * W4<T>::value(next[j]) : 0.0f;
-      if (h + L::SUM_SETS < halves) load_scales(h + L::SUM_SETS);
+      if (h + 1 < halves) load_scales(h + 1);
       if (!wait_of<NT>(done + 8 * slot, slot_phase, abort_flag)) {
         if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
         break;
@@ -310,9 +313,9 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ready + 8 * freed);
-      set = (set + L::SUM_SETS) % SETS, freed = (freed + L::SUM_SETS) % SLOTS;
-      slot += L::SUM_SETS;
-      if (slot >= SLOTS) slot -= SLOTS, slot_phase ^= 1u;
+      if (++set == SETS) set = 0;
+      if (++freed == SLOTS) freed = 0;
+      if (++slot == SLOTS) slot = 0, slot_phase ^= 1u;
     }
   }
 
@@ -321,29 +324,16 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     if (p.epilogue != EPI_NONE) v = w4_activation(v + W4<T>::value(static_cast<const unsigned short*>(p.bias)[n]), p.epilogue);
     static_cast<T*>(p.c)[static_cast<size_t>(m) * p.N + n] = W4<T>::round(v);
   };
-  const int m0 = L::SUM_SETS == 2 ? 0 : warp / 4 * L::SUM_COLS;  // first token of a warp of sums
-  float* red = reinterpret_cast<float*>(smem + L::OFF_RED);
-  int sum_warps = L::SUM_WARPS;
-  if constexpr (L::SUM_SETS == 2) {  // the odd halves' sums to the even ones'
-    if (warp >= 4 && warp < 8) {
-#pragma unroll
-      for (int i = 0; i < L::SUM_COLS; ++i) red[i * ROWS + row] = acc[i];
-    }
-    __syncthreads();
-    sum_warps = 4;
-    if (warp < 4) {
-#pragma unroll
-      for (int i = 0; i < L::SUM_COLS; ++i) acc[i] += red[i * ROWS + row];
-    }
-  }
+  const int m0 = warp / 4 * L::SUM_COLS;  // first token of a warp of sums
   if (p.split == 1) {
-    if (warp < sum_warps && n0 + row < p.N) {
+    if (warp < L::SUM_WARPS && n0 + row < p.N) {
 #pragma unroll
       for (int i = 0; i < L::SUM_COLS; ++i)
         if (m0 + i < p.M) store(m0 + i, n0 + row, acc[i]);
     }
   } else {
-    if (warp < sum_warps) {
+    float* red = reinterpret_cast<float*>(smem + L::OFF_RED);
+    if (warp < L::SUM_WARPS) {
 #pragma unroll
       for (int i = 0; i < L::SUM_COLS; ++i) red[(m0 + i) * ROWS + row] = acc[i];
     }

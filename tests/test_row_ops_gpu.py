@@ -127,6 +127,36 @@ def test_silu(rows, k, dtype, quant):
     check(y, s, silu64(x), quant, SILU_REL, floor=2.0**-115)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_silu_over_the_range_of_the_gate(dtype):
+    """Every gate value of a 16-bit type (of fp32: as many, over the same range), times 1 and -1; infinities and NaN as the formula has them."""
+    g = torch.arange(-32768, 32768, device="cuda").to(torch.int16).view(torch.bfloat16 if dtype == torch.float32 else dtype).to(dtype)
+    x = torch.stack([torch.cat([g, torch.ones_like(g)]), torch.cat([g, -torch.ones_like(g)])])
+    y, none = silu_mul_quant(x, quant_dtype=None)
+    want = silu64(x)
+    assert none is None
+    want = torch.where(torch.isneginf(x[:, : len(g)].double()), torch.nan, want)  # -Inf times 0
+    assert torch.equal(torch.isnan(y), torch.isnan(want))
+    keep = torch.isfinite(want) & (want.abs() < torch.finfo(dtype).max)
+    assert torch.equal(y[~keep & ~torch.isnan(want)].double(), want[~keep & ~torch.isnan(want)])
+    check(torch.where(keep, y, 0.0), None, torch.where(keep, want, 0.0), None, SILU_REL, floor=2.0**-115)
+
+
+@pytest.mark.parametrize("inter", [8200, 12288, 16384, 28672, 32768, 32776])
+@pytest.mark.parametrize("quant", [FP8, torch.int8], ids=["fp8", "int8"])
+def test_many_wide_gated_rows(inter, quant):
+    """More rows than SMs, wider than a row's registers allow two of; strided rows; a row of zeros, NaN and Inf among them."""
+    x = make(300, 2 * inter + 8, torch.bfloat16, inter)[:, : 2 * inter]
+    x[7] = 0.0
+    x[8, 3], x[9, 5], x[9, 6] = float("nan"), float("inf"), float("-inf")
+    y, s = silu_mul_quant(x, quant_dtype=quant)
+    rows = [i for i in range(300) if i not in (8, 9)]
+    check(y[rows], s[rows], silu64(x)[rows], quant, SILU_REL, floor=2.0**-115)
+    for i in (8, 9):
+        ys, ss = silu_mul_quant(x[i : i + 1], quant_dtype=quant)  # one row takes the other kernel
+        assert torch.equal(y[i : i + 1].view(torch.uint8), ys.view(torch.uint8)) and torch.equal(s[i : i + 1], ss)
+
+
 @pytest.mark.parametrize("k", [4096, 1000, 1003])
 @pytest.mark.parametrize("quant", [FP8, torch.int8], ids=["fp8", "int8"])
 def test_rows_of_zeros_nan_inf_and_the_ends_of_the_range(quant, k):

@@ -111,17 +111,19 @@ def test_every_code_and_place_is_exact(group, x):
 
 
 def test_deterministic_and_independent_of_the_batch():
-    a, q, s, z, bias = make(8, 4100, 4096, 128, "bf16", True, 6)
+    """Of up to 4 tokens (integers), and of 5 to 64."""
+    a, q, s, z, bias = make(40, 4100, 4096, 128, "bf16", True, 6)
     fn = compile_w4a16_gemv(N=4100, K=4096, group_size=128, zero_points=True)
-    outs = []
-    for _ in range(3):
-        c = torch.empty(8, 4100, dtype=torch.bfloat16, device="cuda")
-        fn(c, a, q, s, z, None, 8, 4100, torch.cuda.current_stream())
-        outs.append(c)
-    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
-    one = torch.empty(1, 4100, dtype=torch.bfloat16, device="cuda")
-    fn(one, a[5:6].contiguous(), q, s, z, None, 1, 4100, torch.cuda.current_stream())
-    assert torch.equal(one[0], outs[0][5])
+
+    def product(x):
+        c = torch.empty(len(x), 4100, dtype=torch.bfloat16, device="cuda")
+        fn(c, x, q, s, z, None, len(x), 4100, torch.cuda.current_stream())
+        return c
+
+    few, many = product(a[:4]), product(a)
+    assert all(torch.equal(few, product(a[:4])) and torch.equal(many, product(a)) for _ in range(2))
+    assert torch.equal(product(a[3:4].contiguous())[0], few[3])
+    assert torch.equal(product(a[30:38].contiguous()), many[30:38])
 
 
 def test_infinities_and_nan_stay_in_their_token():
@@ -132,6 +134,20 @@ def test_infinities_and_nan_stay_in_their_token():
     fn(c, a, q, s, z, None, 4, 100, torch.cuda.current_stream())
     assert bool(torch.isnan(c[1]).all()) and not bool(torch.isfinite(c[2]).any())
     check(c[[0, 3]], a[[0, 3]], q, s, z, None, 64)
+
+
+@pytest.mark.parametrize("m", [4, 8, 16, 32, 64])
+@pytest.mark.parametrize("n,k,group", [(28672, 2048, 128), (1024, 16384, 64), (19000, 4096, 32)])
+def test_many_launches_in_a_row(n, k, group, m):
+    """Without a pause between them, more blocks than SMs, weights that come from memory: every one gives the same result."""
+    a, q, s, z, _ = make(m, n, k, group, "fp16", True, 12)
+    fn = compile_w4a16_gemv(N=n, K=k, group_size=group, in_dtype="fp16", zero_points=True)
+    others = [q.clone() for _ in range(4)]
+    outs = [torch.empty(m, n, dtype=torch.float16, device="cuda") for _ in range(40)]
+    for i, c in enumerate(outs):
+        fn(c, a, others[i % 4], s, z, None, m, n, torch.cuda.current_stream())
+    check(outs[0], a, q, s, z, None, group)
+    assert all(torch.equal(outs[0], c) for c in outs)
 
 
 @pytest.mark.parametrize("m", [1, 4, 5, 40])
