@@ -271,7 +271,9 @@ __device__ __forceinline__ void norm_stats(const float (&h)[N], const float (&w)
   }
 }
 
-// Single pass: the row's NV vectors per thread stay in registers, all loads of a thread are in flight together.
+// Single pass: the row's NV vectors per thread stay in registers, all loads of a thread are in flight together.  16384 x 8192 bf16 with
+// residual to fp8: 212 us with the sums as they were read and read twice, 185 with h w in fp32 between the passes and packed additions, 170 with
+// two vectors a thread in place of four (64 registers and spills); floor 144.
 template <typename T, int Q, int NV>
 __global__ void __launch_bounds__(NV == 8 ? 512 : 1024) rmsnorm_row_kernel(RowParams p) {
   constexpr int N = VEC_OF<T>;
@@ -549,7 +551,8 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
 // Per-row scale of wide rows, many of them: a row in registers is more than half of an SM's, so there is no second block whose loads
 // could go on while this one reduces, converts and stores.  Here a warp of its own brings the rows, chunk by chunk and over
 // their ends, into a ring in shared memory by bulk copies; the others take a vector of every chunk per thread.
-// us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, RING_TIME here (floor 180).
+// us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, 267 here, 247 with one barrier a row and the exponential above (floor
+// 180).  Bound: issue slots (71 % busy, DRAM at 64 % of the copy rate).
 constexpr int RING_WARPS = 16, RING_THREADS = 32 * RING_WARPS;
 constexpr int RING_CHUNK = 16 * RING_THREADS;                   // bytes of gate values, and as many of up values
 constexpr int RING_SLOTS = 13;
