@@ -551,8 +551,9 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
 // Per-row scale of wide rows, many of them: a row in registers is more than half of an SM's, so there is no second block whose loads
 // could go on while this one reduces, converts and stores.  Here a warp of its own brings the rows, chunk by chunk and over
 // their ends, into a ring in shared memory by bulk copies; the others take a vector of every chunk per thread.
-// us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, 267 here, 247 with one barrier a row and the exponential above (floor
-// 180).  Bound: issue slots (71 % busy, DRAM at 64 % of the copy rate).
+// us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, 267 here, 243 with one barrier a row, the exponential above and
+// waits that look before they sleep (floor 180).  Bound: issue slots and the pauses between rows (71 % busy); an exponential of five
+// instructions less changes nothing.
 constexpr int RING_WARPS = 16, RING_THREADS = 32 * RING_WARPS;
 constexpr int RING_CHUNK = 16 * RING_THREADS;                   // bytes of gate values, and as many of up values
 constexpr int RING_SLOTS = 13;
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(RING_THREADS + 32, 1) silu_ring_kernel(RowPara
     float v[NV][N], mx = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (ok && !mbar_wait_warp(full + 8 * slot, phase, abort_flag)) {
+      if (ok && !mbar_wait_soon(full + 8 * slot, phase, abort_flag)) {
         if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
         ok = false;
       }

