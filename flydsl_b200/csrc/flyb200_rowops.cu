@@ -36,7 +36,6 @@ struct RowParams {
   int warps_per_row;
   int w_f32;        // the weight is fp32, whatever x is
   float eps;
-  int* status;      // of bounded waits (wide gated rows)
 };
 
 template <typename T>
@@ -549,85 +548,62 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
 }
 
 // Per-row scale of wide rows, many of them: a row in registers is more than half of an SM's, so there is no second block whose loads
-// could go on while this one reduces, converts and stores.  Here a warp of its own brings the rows, chunk by chunk and over
-// their ends, into a ring in shared memory by bulk copies; the others take a vector of every chunk per thread.
-// us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, 267 here, 243 with one barrier a row, the exponential above and
-// waits that look before they sleep (floor 180).  Bound: issue slots and the pauses between rows (71 % busy); an exponential of five
-// instructions less changes nothing.
-constexpr int RING_WARPS = 16, RING_THREADS = 32 * RING_WARPS;
-constexpr int RING_CHUNK = 16 * RING_THREADS;                   // bytes of gate values, and as many of up values
+// could go on while this one reduces, converts and stores.  Here the loads run ahead of all that, over the ends of rows: every thread copies its own
+// vectors into a ring in shared memory and reads them back itself, so that nothing but its own wait stands between the two - no
+// barrier, no flag, no other thread.  us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, 232 here; 250 to 262 with a warp of its own that
+// filled the ring by bulk copies (floor 180).
+constexpr int RING_THREADS = 512, RING_WARPS = RING_THREADS / 32;
+constexpr int RING_CHUNK = 16 * RING_THREADS;  // bytes of gate values, and as many of up values: a vector of each per thread
 constexpr int RING_SLOTS = 13;
-constexpr int RING_BYTES = RING_SLOTS * 2 * RING_CHUNK + 512;
+constexpr int RING_BYTES = RING_SLOTS * 2 * RING_CHUNK;
+
+__device__ __forceinline__ void copy16_once(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+}
 
 template <typename T, int Q, int NV>
-__global__ void __launch_bounds__(RING_THREADS + 32, 1) silu_ring_kernel(RowParams p) {
+__global__ void __launch_bounds__(RING_THREADS, 1) silu_ring_kernel(RowParams p) {
   constexpr int N = VEC_OF<T>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float reds[3][64];  // of even rows, of odd rows, of the second maximum
-  const int warp = warp_index(), lane = threadIdx.x & 31, tid = threadIdx.x;
-  const uint32_t base = smem_u32(smem), full = base + RING_SLOTS * 2 * RING_CHUNK + 16, empty = full + 8 * RING_SLOTS;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + RING_SLOTS * 2 * RING_CHUNK);
-  if (tid == 0) {
-    for (int i = 0; i < RING_SLOTS; ++i) {
-      mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, RING_WARPS);
-    }
-    abort_flag[0] = 0;
-    abort_flag[1] = 0;
-    fence_mbar_init();
-  }
-  __syncthreads();
+  const int tid = threadIdx.x;
+  const uint8_t* mine = smem + tid * 16;
+  const uint32_t base = smem_u32(mine);
   pdl_wait(p.x, p.y, p.scale);
   pdl_trigger();
-  int slot = 0;
-  uint32_t phase = 0;
-  if (warp == RING_WARPS) {
-    const bool issuer = elect_one();
-    const uint64_t once = l2_policy_evict_first();
-    int issued = 0;
-    bool ok = true;
-    for (long long row = blockIdx.x; row < p.rows && ok; row += gridDim.x) {
-      const T* xr = static_cast<const T*>(p.x) + row * p.x_stride;
-      for (int k = 0; k < p.width; k += RING_THREADS * N) {
-        if (!mbar_wait_warp(empty + 8 * slot, phase ^ 1u, abort_flag)) {
-          report_failure(p.status, ST_TIMEOUT, abort_flag);
-          ok = false;
-          break;
-        }
-        if (issuer) {
-          const uint32_t bytes = min(RING_THREADS * N, p.width - k) * static_cast<int>(sizeof(T)), at = base + slot * 2 * RING_CHUNK;
-          mbar_expect_tx(full + 8 * slot, 2 * bytes);
-          bulk_load_1d(at, xr + k, bytes, full + 8 * slot, once);
-          bulk_load_1d(at + RING_CHUNK, xr + p.width + k, bytes, full + 8 * slot, once);
-        }
-        ++issued;
-        if (++slot == RING_SLOTS) slot = 0, phase ^= 1u;
+  const uint64_t once = l2_policy_evict_first();
+
+  long long ahead_row = blockIdx.x;
+  int ahead_k = tid * N, ahead_slot = 0;
+  auto copy_next = [&]() {  // one group, empty behind the last row and for threads behind a row's end
+    if (ahead_row < p.rows) {
+      if (ahead_k < p.width) {
+        const T* from = static_cast<const T*>(p.x) + ahead_row * p.x_stride + ahead_k;
+        const uint32_t at = base + ahead_slot * 2 * RING_CHUNK;
+        copy16_once(at, from, once);
+        copy16_once(at + RING_CHUNK, from + p.width, once);
+      }
+      ahead_k += RING_THREADS * N;
+      if (ahead_k >= NV * RING_THREADS * N) {
+        ahead_k = tid * N;
+        ahead_row += gridDim.x;
       }
     }
-    if (!ok || *abort_flag) {  // copies in flight land before the block leaves
-      const int pending = min(issued, RING_SLOTS);
-      for (int i = 0; i < pending; ++i) {
-        int s = slot - 1 - i;
-        uint32_t ph = phase;
-        if (s < 0) s += RING_SLOTS, ph ^= 1u;
-        mbar_wait(full + 8 * s, ph, abort_flag + 1);
-      }
-    }
-    return;
-  }
-  bool ok = true;  // a warp that gave up goes on through the barriers without waiting
-  int odd = 0;
+    if (++ahead_slot == RING_SLOTS) ahead_slot = 0;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int i = 0; i < RING_SLOTS - 1; ++i) copy_next();
+
+  int slot = 0, odd = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     float v[NV][N], mx = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (ok && !mbar_wait_soon(full + 8 * slot, phase, abort_flag)) {
-        if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
-        ok = false;
-      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(RING_SLOTS - 2) : "memory");  // the oldest one is here
       if ((i * RING_THREADS + tid) * N < p.width) {
         float u[N];
-        const uint8_t* at = smem + slot * 2 * RING_CHUNK + tid * 16;
+        const uint8_t* at = mine + slot * 2 * RING_CHUNK;
         unpack(load_raw<T, N>(reinterpret_cast<const T*>(at)), v[i]);
         unpack(load_raw<T, N>(reinterpret_cast<const T*>(at + RING_CHUNK)), u);
 #pragma unroll
@@ -636,9 +612,8 @@ __global__ void __launch_bounds__(RING_THREADS + 32, 1) silu_ring_kernel(RowPara
           mx = max_abs(mx, v[i][j]);
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + 8 * slot);
-      if (++slot == RING_SLOTS) slot = 0, phase ^= 1u;
+      if (++slot == RING_SLOTS) slot = 0;
+      copy_next();  // over the slot that was read one time earlier
     }
     row_reduce<false, true>(none, mx, RING_WARPS, 0, 1, reds[odd]);  // nobody writes over it before all are at the next row's barrier
     odd ^= 1;
@@ -675,6 +650,7 @@ __global__ void __launch_bounds__(RING_THREADS + 32, 1) silu_ring_kernel(RowPara
       }
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Per-row scale of any row: two or three passes that compute the values again.
@@ -805,10 +781,9 @@ cudaError_t launch_silu_ring(RowParams p, cudaStream_t s) {
     if (cudaError_t e = cudaFuncSetAttribute(silu_ring_kernel<T, Q, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES)) return e;
     done.fetch_or(bit, std::memory_order_release);
   }
-  if (host::status_word(&p.status)) return cudaErrorInvalidDevice;
   int sms = 0;
   if (host::sm_count(&sms)) return cudaErrorInvalidDevice;
-  return host::launch_dependent(silu_ring_kernel<T, Q, NV>, dim3(p.rows < sms ? p.rows : sms), RING_THREADS + 32, RING_BYTES, s, p);
+  return host::launch_dependent(silu_ring_kernel<T, Q, NV>, dim3(p.rows < sms ? p.rows : sms), RING_THREADS, RING_BYTES, s, p);
 }
 
 template <typename T, int Q>
@@ -883,7 +858,7 @@ int flyb200_rmsnorm_quant(void* y, void* scale, void* residual_out, const void* 
   bool vectors = K % n == 0 && x_stride % n == 0 && multiple(x, 16) && multiple(weight, 16) && multiple(y, quant == Q_NONE ? 16 : n);
   if (residual)
     vectors = vectors && residual_stride % n == 0 && residual_out_stride % n == 0 && multiple(residual, 16) && multiple(residual_out, 16);
-  const RowParams p = {y, scale, residual_out, x, residual, weight, x_stride, residual_stride, residual_out_stride, rows, K, 0, weight_f32 ? 1 : 0, eps, nullptr};
+  const RowParams p = {y, scale, residual_out, x, residual, weight, x_stride, residual_stride, residual_out_stride, rows, K, 0, weight_f32 ? 1 : 0, eps};
   CUDA_TRY(launch_rows<true>(p, x_dtype, quant, vectors, static_cast<cudaStream_t>(stream)));
   return FLYB200_OK;
 }
@@ -897,7 +872,7 @@ int flyb200_silu_mul_quant(void* y, void* scale, const void* x, int rows, int in
   if (!multiple(x, e) || !multiple(y, quant == Q_NONE ? e : 1) || (quant != Q_MXFP8 && !multiple(scale, 4))) return FLYB200_E_BAD_ALIGN;
   if (rows == 0) return FLYB200_OK;
   const bool vectors = inter % n == 0 && x_stride % n == 0 && multiple(x, 16) && multiple(y, quant == Q_NONE ? 16 : n);
-  const RowParams p = {y, scale, nullptr, x, nullptr, nullptr, x_stride, 0, 0, rows, inter, 0, 0, 0.0f, nullptr};
+  const RowParams p = {y, scale, nullptr, x, nullptr, nullptr, x_stride, 0, 0, rows, inter, 0, 0, 0.0f};
   if (quant == Q_NONE || quant == Q_MXFP8) {
     const long long blocks = ((vectors ? inter / n : inter) + 255ll) / 256 * rows;
     if (blocks > 0x7fffffffll) return FLYB200_E_UNSUPPORTED;
