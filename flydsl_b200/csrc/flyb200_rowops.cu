@@ -188,10 +188,11 @@ __device__ __forceinline__ RowScale row_scale(float m, float f) {
   o.low = fmaf(-o.mul, m, m > 0.0f ? QMAX_OF<Q> : 0.0f) * (o.mul * (1.0f / QMAX_OF<Q>));
   return o;
 }
-// Whether the short form above holds: finite, and neither the maximum nor the scale near the lower end of fp32.
+// Whether the short form above holds: finite, and neither the maximum nor the scale near the lower end of fp32.  A row of zeros with an
+// infinite f (no eps) is 0 times infinity.
 template <int Q>
 __device__ __forceinline__ bool row_is_plain(float m, float f) {
-  return m == 0.0f || (m >= 1e-30f && m < INFINITY && f > 0.0f && m * f >= 1e-30f && m * f < INFINITY);
+  return m == 0.0f ? f < INFINITY : m >= 1e-30f && m < INFINITY && f > 0.0f && m * f >= 1e-30f && m * f < INFINITY;
 }
 
 // N codes of values already multiplied into code units; int8: the nearest integer by adding 1.5 * 2^23, whose last bits are

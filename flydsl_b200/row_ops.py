@@ -97,7 +97,8 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 def rmsnorm_quant(x, weight, eps=1e-6, *, residual=None, quant_dtype=torch.float8_e4m3fn, residual_out=None):
     """``(y, scale, h)``: ``h = x + residual`` rounded to x's type, and the codes and scales of
     ``h * weight / sqrt(mean(h^2) + eps)`` over the last dimension, statistics and values in fp32 (squares beyond its range
-    are infinite, and such a row is all zeros).  ``weight`` [K] is of x's type or fp32.  Without a residual ``h`` is None.
+    are infinite, and such a row is all zeros; squares below it are 0, and without ``eps`` the values of such a row are infinite, or NaN where
+    they are 0).  ``weight`` [K] is of x's type or fp32.  Without a residual ``h`` is None.
     ``residual_out`` receives ``h`` instead of a new tensor; it may be ``residual`` (or ``x``) itself, for an update in place,
     and must not overlap them otherwise."""
     quant = _code(quant_dtype)

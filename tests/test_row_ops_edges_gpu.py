@@ -3,8 +3,8 @@
 import pytest
 import torch
 
-from flydsl_b200 import silu_mul_quant
-from tests.test_row_ops_gpu import FP8, SILU_REL, TYPES, check, make, silu64
+from flydsl_b200 import rmsnorm_quant, silu_mul_quant
+from tests.test_row_ops_gpu import FP8, SILU_REL, TYPES, check, make, norm64, norm_rel, silu64
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +22,26 @@ def test_many_wide_gated_rows_of_every_type(vectors, dtype, quant):
     for i in (0, 5, 300):
         ys, ss = silu_mul_quant(x[i : i + 1], quant_dtype=quant)  # one row takes the other kernel
         assert torch.equal(y[i : i + 1].view(torch.uint8), ys.view(torch.uint8)) and torch.equal(s[i : i + 1], ss)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-60])
+@pytest.mark.parametrize("k", [4096, 1003, 40000])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("quant", [FP8, torch.int8], ids=["fp8", "int8"])
+def test_zero_rows_without_eps(quant, dtype, k, eps):
+    """A row of zeros is 0 / 0 in every place, that is NaN, that is 0 with scale 1.  Squares below fp32 are 0: the values are infinite
+    then, so qmax with scale 1 (to the rounding of qmax * (1 / qmax)), or NaN and so 0 where the weight is 0."""
+    x = make(8, k, dtype, 40)
+    w = make(1, k, dtype, 41)[0].abs() + 0.5
+    x[2] = 0.0
+    qmax = 448.0 if quant == FP8 else 127.0
+    if dtype != torch.float16:  # 1e-25 is 0 in fp16
+        x[5] = 1e-25
+    y, s, _ = rmsnorm_quant(x, w, eps, quant_dtype=quant)
+    assert not bool(y[2].float().any()) and float(s[2]) == 1.0
+    if dtype != torch.float16:
+        assert bool((y[5].float() == qmax).all()) and abs(float(s[5]) - 1.0) <= 2.0**-23
+    good = [0, 1, 3, 4, 6, 7]
+    check(y[good], s[good], norm64(x, w, 0.0)[0][good], quant, norm_rel(k))
+    y, s, h = rmsnorm_quant(x, torch.zeros_like(w), eps, residual=torch.zeros_like(x), quant_dtype=quant)
+    assert not bool(y.float().any()) and bool((s == 1.0).all()) and torch.equal(h, x)
