@@ -5,11 +5,22 @@ statements take the call, an int for a library code."""
 
 from __future__ import annotations
 
+import torch
+
 from . import _lib
+
+_key = torch._C._dispatch_key_parse
+_WRAPPED = [_key(k) for k in ("Python", "PythonTLSSnapshot", "Functionalize", "Negative", "Conjugate", "ZeroTensor", "FuncTorchBatched",
+                              "FuncTorchGradWrapper", "BatchedNestedTensor", "Batched")]
+_WATCHING = [_key(k) for k in ("Python", "PythonTLSSnapshot", "Functionalize", "FuncTorchDynamicLayerFrontMode", "FuncTorchVmapMode", "VmapMode",
+                               "Tracer", "PreDispatch", "PythonDispatcher")]
 
 
 def eager(x) -> bool:
-    return False
+    if type(x) not in (torch.Tensor, torch.nn.Parameter):
+        return False
+    keys, on = torch._C._dispatch_keys(x), torch._C._dispatch_tls_local_include_set()
+    return not any(keys.has(k) for k in _WRAPPED) and not any(on.has(k) for k in _WATCHING)
 
 
 def _left_to_the_caller(*args):

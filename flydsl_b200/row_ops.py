@@ -16,15 +16,18 @@ so they can be captured into a CUDA graph.  ``quant_dtype`` says what comes out:
 ``None``      the values rounded to the type of x, scale ``None``: for projections on 16-bit activations.
 
 Inputs are CUDA tensors of fp32, fp16 or bf16 whose last dimension is contiguous; rows may lie further apart than they are
-long (a slice of a wider tensor).  Anything else raises ``ValueError``, as do inputs that carry a gradient: the operators
-have no backward pass.
+long (a slice of a wider tensor).  Anything else raises ``ValueError``, as do inputs that carry a gradient, backward or forward: the
+operators have no derivative.  Where torch has to see the operations (tracing and compilation, fake tensors and other subclasses, dispatch
+modes, functional transforms, lazily negated tensors) they run as torch operations, with the same results up to the last places.
 """
 
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad
 
 from . import _lib
+from .kernels.gemm.mxfp8_preshuffle import per_1x32_f8_quant_torch
 
 _X_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _QUANT = {None: _lib.ROWQ_NONE, torch.float8_e4m3fn: _lib.ROWQ_FP8, torch.int8: _lib.ROWQ_INT8, "mxfp8": _lib.ROWQ_MXFP8}
@@ -37,6 +40,18 @@ def _code(quant_dtype) -> int:
     return q
 
 
+def _no_tangent(name: str, t: torch.Tensor) -> None:
+    if torch.compiler.is_compiling() or torch.autograd.forward_ad._current_level < 0:
+        return
+    if torch.autograd.forward_ad.unpack_dual(t, level=0).tangent is not None:
+        raise ValueError(f"{name} carries a tangent, and this operator has no forward derivative")
+
+
+def _watched(*tensors) -> bool:
+    """Whether torch has to see the operations on these tensors: no kernel may stand for them."""
+    return torch.compiler.is_compiling() or not all(_lib.ops().eager(t) for t in tensors if t is not None)
+
+
 def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> tuple[int, int]:
     """(rows, stride between them in elements) of a tensor [..., K] with rows at equal distances."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.layout != torch.strided or t.dtype not in _X_DTYPES or t.dim() < 1:
@@ -45,6 +60,7 @@ def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> tuple
         raise ValueError(f"{name} must have the shape, dtype and device of x")
     if torch.is_grad_enabled() and t.requires_grad:
         raise ValueError(f"{name} requires a gradient, and this operator has no backward pass: call it under torch.no_grad()")
+    _no_tangent(name, t)
     k = t.shape[-1]
     if k == 0:
         raise ValueError(f"{name} has rows without elements")
@@ -94,6 +110,20 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _quantised(v: torch.Tensor, dtype: torch.dtype, quant: int):
+    """The outputs of fp32 values as torch operations."""
+    if quant == _lib.ROWQ_NONE:
+        return v.to(dtype), None
+    if quant == _lib.ROWQ_MXFP8:
+        return per_1x32_f8_quant_torch(v)
+    qmax = 127.0 if quant == _lib.ROWQ_INT8 else 448.0
+    v = torch.nan_to_num(v, nan=0.0, posinf=qmax, neginf=-qmax)
+    s = v.abs().amax(dim=-1, keepdim=True) * (1.0 / qmax)
+    s = torch.where(s == 0, torch.ones_like(s), s)
+    q = (v / s).clamp(-qmax, qmax)
+    return (q.round().to(torch.int8) if quant == _lib.ROWQ_INT8 else q.to(torch.float8_e4m3fn)), s
+
+
 def rmsnorm_quant(x, weight, eps=1e-6, *, residual=None, quant_dtype=torch.float8_e4m3fn, residual_out=None):
     """``(y, scale, h)``: ``h = x + residual`` rounded to x's type, and the codes and scales of
     ``h * weight / sqrt(mean(h^2) + eps)`` over the last dimension, statistics and values in fp32 (squares beyond its range
@@ -107,11 +137,12 @@ def rmsnorm_quant(x, weight, eps=1e-6, *, residual=None, quant_dtype=torch.float
         raise ValueError(f"eps must not be negative, got {eps}")
     if residual is None and residual_out is not None:
         raise ValueError("residual_out without a residual")
-    r = _lib.ops().rmsnorm_quant(x, weight, residual, residual_out, eps, quant)
-    if type(r) is tuple:
-        return r
-    if type(r) is int:
-        _lib.check(r, "rmsnorm_quant")
+    if not torch.compiler.is_compiling():
+        r = _lib.ops().rmsnorm_quant(x, weight, residual, residual_out, eps, quant)
+        if type(r) is tuple:
+            return r
+        if type(r) is int:
+            _lib.check(r, "rmsnorm_quant")
     # not the common form: the same step by step, with what is wrong by name
     rows, stride = _rows("x", x)
     k = x.shape[-1]
@@ -121,20 +152,29 @@ def rmsnorm_quant(x, weight, eps=1e-6, *, residual=None, quant_dtype=torch.float
         raise ValueError(f"weight must be {x.dtype} or fp32, got {weight.dtype}")
     if torch.is_grad_enabled() and weight.requires_grad:
         raise ValueError("weight requires a gradient, and this operator has no backward pass: call it under torch.no_grad()")
+    _no_tangent("weight", weight)
+    watched = _watched(x, weight, residual, residual_out)
     r_stride = h_stride = 0
     h = None
     if residual is not None:
         r_stride = _rows("residual", residual, x)[1]
         h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual_out is None else residual_out
         h_stride = _rows("residual_out", h, x)[1]
-        for name, t in (("x", x), ("residual", residual)):
+        for name, t in (("x", x), ("residual", residual)) if not watched else ():
             if residual_out is not None and _overlap(h, t) and (h.data_ptr() != t.data_ptr() or h.stride() != t.stride()):
                 raise ValueError(f"residual_out overlaps {name} without being the same tensor")
-        if residual_out is not None and _overlap(h, weight):
+        if residual_out is not None and not watched and _overlap(h, weight):
             raise ValueError("residual_out overlaps weight")
     y, scale = _outputs(x, k, quant)
     if rows == 0:
         return y, scale, h
+    if watched:
+        if residual is not None:
+            x = (x.float() + residual.float()).to(x.dtype)
+            h = x if residual_out is None else residual_out.copy_(x)
+        v = x.float()
+        v = v * torch.rsqrt(v.square().mean(dim=-1, keepdim=True) + eps) * weight.float()
+        return *_quantised(v, x.dtype, quant), h
     with _lib.on_device(x.device):
         rc = _lib.load().flyb200_rmsnorm_quant(
             y.data_ptr(), None if scale is None else scale.data_ptr(), None if h is None else h.data_ptr(), x.data_ptr(),
@@ -149,11 +189,12 @@ def silu_mul_quant(x, *, quant_dtype=torch.float8_e4m3fn):
     """``(y, scale)``: codes and scales of ``silu(gate) * up`` for ``x = [..., 2 * inter]``, of every row the gate values
     first (the row order of a gate-up projection's weights), values in fp32."""
     quant = _code(quant_dtype)
-    r = _lib.ops().silu_mul_quant(x, quant)
-    if type(r) is tuple:
-        return r
-    if type(r) is int:
-        _lib.check(r, "silu_mul_quant")
+    if not torch.compiler.is_compiling():
+        r = _lib.ops().silu_mul_quant(x, quant)
+        if type(r) is tuple:
+            return r
+        if type(r) is int:
+            _lib.check(r, "silu_mul_quant")
     rows, stride = _rows("x", x)
     if x.shape[-1] % 2 != 0:
         raise ValueError(f"x needs an even last dimension (gate and up values), got {x.shape[-1]}")
@@ -161,6 +202,9 @@ def silu_mul_quant(x, *, quant_dtype=torch.float8_e4m3fn):
     y, scale = _outputs(x, inter, quant)
     if rows == 0:
         return y, scale
+    if _watched(x):
+        g, u = x.float().chunk(2, dim=-1)
+        return _quantised(g / (1.0 + torch.exp(-g)) * u, x.dtype, quant)
     with _lib.on_device(x.device):
         rc = _lib.load().flyb200_silu_mul_quant(y.data_ptr(), None if scale is None else scale.data_ptr(), x.data_ptr(), rows, inter, stride,
                                                 _X_DTYPES[x.dtype], quant, _lib.current_stream(x.device))
