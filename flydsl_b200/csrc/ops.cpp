@@ -104,18 +104,22 @@ T* as(const at::Tensor& t) {
   return static_cast<T*>(ptr(t));
 }
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-// Whether a kernel may stand for torch operations on the tensor `o`: a plain tensor (no subclass, fake,
-// functionalised, functorch-wrapped, lazily negated or conjugated one), with no dispatch mode, trace or transform
-// in force that has to see the operations.  `differentiable`: nor a gradient that they would carry.
-bool runs_eagerly(PyObject* o, bool differentiable) {
+// Whether the memory of `t` holds its values (no fake, functionalised, functorch-wrapped, lazily negated or conjugated tensor, no
+// subclass with a dispatch of its own), with no dispatch mode, trace or transform in force that has to see what is done with them.
+bool readable(const at::Tensor& t) {
   using K = c10::DispatchKey;
   constexpr c10::DispatchKeySet wrapped({K::Python, K::PythonTLSSnapshot, K::Functionalize, K::Negative, K::Conjugate, K::ZeroTensor,
                                          K::FuncTorchBatched, K::FuncTorchGradWrapper, K::BatchedNestedTensor, K::Batched});
   constexpr c10::DispatchKeySet watching({K::Python, K::PythonTLSSnapshot, K::Functionalize, K::FuncTorchDynamicLayerFrontMode,
                                           K::FuncTorchVmapMode, K::VmapMode, K::Tracer, K::PreDispatch, K::PythonDispatcher});
+  return !t.key_set().has_any(wrapped) && !c10::impl::tls_local_dispatch_key_set().included_.has_any(watching);
+}
+// Whether a kernel may stand for torch operations on the tensor `o`: readable, and no subclass.  `differentiable`: nor a
+// gradient that the operations would carry.
+bool runs_eagerly(PyObject* o, bool differentiable) {
   if (!THPVariable_CheckExact(o)) return false;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (t.key_set().has_any(wrapped) || c10::impl::tls_local_dispatch_key_set().included_.has_any(watching)) return false;
+  if (!readable(t)) return false;
   return !differentiable || !((c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined());
 }
 void* handle(long long s) { return reinterpret_cast<void*>(static_cast<uintptr_t>(s)); }
@@ -269,6 +273,8 @@ PyObject* w4_gemv(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   const int M = a.i32(), N = a.i32(), K = a.i32(), group = a.i32(), dtype = a.i32(), epi = a.i32();
   const long long s = a.integer();
   if (!a.done() || M <= 0 || N <= 0 || K <= 0 || group <= 0) return none();
+  for (const at::Tensor* v : {&c, &x, &q, &scale, &zero, &bias})
+    if (v->defined() && (!readable(*v) || v->_fw_grad(0).defined())) return none();
   const at::ScalarType t = dtype == FLYB200_DT_FP16 ? at::kHalf : at::kBFloat16;
   const long long m = M, nn = N, k = K, groups = nn * (k / group);
   auto fits = [&](const at::Tensor& v, long long least) { return plain(v) && v.scalar_type() == t && v.numel() >= least && v.device() == c.device(); };

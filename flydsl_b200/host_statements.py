@@ -16,11 +16,13 @@ _WATCHING = [_key(k) for k in ("Python", "PythonTLSSnapshot", "Functionalize", "
                                "Tracer", "PreDispatch", "PythonDispatcher")]
 
 
-def eager(x) -> bool:
-    if type(x) not in (torch.Tensor, torch.nn.Parameter):
-        return False
+def _readable(x) -> bool:
     keys, on = torch._C._dispatch_keys(x), torch._C._dispatch_tls_local_include_set()
     return not any(keys.has(k) for k in _WRAPPED) and not any(on.has(k) for k in _WATCHING)
+
+
+def eager(x) -> bool:
+    return type(x) in (torch.Tensor, torch.nn.Parameter) and _readable(x)
 
 
 def _left_to_the_caller(*args):

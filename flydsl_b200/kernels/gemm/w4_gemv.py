@@ -18,7 +18,10 @@ may depend on the number of tokens.
 
 Any number of tokens runs, in blocks of 64 that each stream the weights; for more than that the 8-bit products
 on the tensor core (``compile_preshuffle_gemm``) are the faster ones.  Weights, activations and scales are read in place, on
-the stream given; nothing is kept between calls, so a launch can be captured into a CUDA graph.
+the stream given; nothing is kept between calls, so a launch can be captured into a CUDA graph.  ``c`` must not overlap the inputs.
+As with the other launchers no gradient is recorded.  Where torch has to see the operations (tracing and compilation, dispatch modes, functional
+transforms, fake tensors, lazily negated tensors, subclasses with a dispatch of their own, tangents) the launch runs as torch operations on torch's
+current stream, with the weights in fp32.
 """
 
 from __future__ import annotations
@@ -28,10 +31,17 @@ import os
 import torch
 
 from ... import _lib
+from ...utils import has_tangent, readable
 from .preshuffle_gemm import _stream_handle
 
 _TORCH = {"bf16": torch.bfloat16, "fp16": torch.float16}
 GROUP_SIZES = (32, 64, 128)
+_ACTIVATIONS = {
+    "bias": lambda v: v,
+    "bias_relu": torch.relu,
+    "bias_silu": torch.nn.functional.silu,
+    "bias_gelu": lambda v: torch.nn.functional.gelu(v, approximate="tanh"),
+}
 
 
 def per_group_w4_quant(w: torch.Tensor, group_size: int = 128, *, zero_points: bool = False, scale_dtype: torch.dtype | None = None):
@@ -90,10 +100,15 @@ class W4Gemv:
             raise ValueError("zero_b is missing: the launcher was built with zero_points=True")
         zero = arg_zero_b if self.zero_points else None
         bias = arg_bias if self._epi else None
-        s = _stream_handle(stream)
-        rc = _lib.ops().w4_gemv(arg_c, arg_a, arg_b, arg_scale_b, zero, bias, M, self.N, self.K, self.group_size, self._dt, self._epi, s)
+        rc = None
+        if not torch.compiler.is_compiling():
+            s = _stream_handle(stream)
+            rc = _lib.ops().w4_gemv(arg_c, arg_a, arg_b, arg_scale_b, zero, bias, M, self.N, self.K, self.group_size, self._dt, self._epi, s)
         if rc is None:
-            self._check(arg_c, arg_a, arg_b, arg_scale_b, zero, bias, M)
+            tensors = (arg_c, arg_a, arg_b, arg_scale_b, zero, bias)
+            self._check(*tensors, M)
+            if not readable(*tensors) or any(has_tangent(t) for t in tensors if t is not None):
+                return self._statements(*tensors, M)
             with _lib.on_device(arg_c.device):
                 rc = _lib.load().flyb200_gemv_w4a16(
                     arg_c.data_ptr(), arg_a.data_ptr(), arg_b.data_ptr(), arg_scale_b.data_ptr(), None if zero is None else zero.data_ptr(),
@@ -102,6 +117,16 @@ class W4Gemv:
         if rc:
             _lib.check(rc, "w4a16_gemv")
         return None
+
+    def _statements(self, c, a, b, scale, zero, bias, M):
+        groups = self.K // self.group_size
+        codes = b.reshape(-1)[: self.N * self.K // 2].view(torch.uint8).reshape(self.N, self.K // 2)
+        z = None if zero is None else zero.reshape(-1)[: self.N * groups].reshape(self.N, groups)
+        w = w4_to_f32(codes, scale.reshape(-1)[: self.N * groups].reshape(self.N, groups), z)
+        v = a.reshape(-1)[: M * self.K].reshape(M, self.K).float() @ w.t()
+        if self._epi:
+            v = _ACTIVATIONS[self.epilogue](v + bias.reshape(-1)[: self.N].float())
+        c.view(-1)[: M * self.N].copy_(v.reshape(-1))
 
     def _check(self, c, a, b, scale, zero, bias, M):
         t16, groups = _TORCH[self.in_dtype], self.K // self.group_size

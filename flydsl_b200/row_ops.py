@@ -24,10 +24,10 @@ modes, functional transforms, lazily negated tensors) they run as torch operatio
 from __future__ import annotations
 
 import torch
-import torch.autograd.forward_ad
 
 from . import _lib
 from .kernels.gemm.mxfp8_preshuffle import per_1x32_f8_quant_torch
+from .utils import has_tangent, readable, torch_watches
 
 _X_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _QUANT = {None: _lib.ROWQ_NONE, torch.float8_e4m3fn: _lib.ROWQ_FP8, torch.int8: _lib.ROWQ_INT8, "mxfp8": _lib.ROWQ_MXFP8}
@@ -41,15 +41,8 @@ def _code(quant_dtype) -> int:
 
 
 def _no_tangent(name: str, t: torch.Tensor) -> None:
-    if torch.compiler.is_compiling() or torch.autograd.forward_ad._current_level < 0:
-        return
-    if torch.autograd.forward_ad.unpack_dual(t, level=0).tangent is not None:
+    if has_tangent(t):
         raise ValueError(f"{name} carries a tangent, and this operator has no forward derivative")
-
-
-def _watched(*tensors) -> bool:
-    """Whether torch has to see the operations on these tensors: no kernel may stand for them."""
-    return torch.compiler.is_compiling() or not all(_lib.ops().eager(t) for t in tensors if t is not None)
 
 
 def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> tuple[int, int]:
@@ -153,7 +146,7 @@ def rmsnorm_quant(x, weight, eps=1e-6, *, residual=None, quant_dtype=torch.float
     if torch.is_grad_enabled() and weight.requires_grad:
         raise ValueError("weight requires a gradient, and this operator has no backward pass: call it under torch.no_grad()")
     _no_tangent("weight", weight)
-    watched = _watched(x, weight, residual, residual_out)
+    watched = torch_watches(x, residual, residual_out) or not readable(weight)
     r_stride = h_stride = 0
     h = None
     if residual is not None:
@@ -202,7 +195,7 @@ def silu_mul_quant(x, *, quant_dtype=torch.float8_e4m3fn):
     y, scale = _outputs(x, inter, quant)
     if rows == 0:
         return y, scale
-    if _watched(x):
+    if torch_watches(x):
         g, u = x.float().chunk(2, dim=-1)
         return _quantised(g / (1.0 + torch.exp(-g)) * u, x.dtype, quant)
     with _lib.on_device(x.device):

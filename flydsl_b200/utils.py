@@ -12,10 +12,29 @@ tensors it runs the library's permutation kernel.
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad
 
-from . import _lib
+from . import _lib, host_statements
 
 _FP8_TYPES = tuple(getattr(torch, n) for n in ("float8_e4m3fn", "float8_e4m3fnuz", "float8_e5m2") if hasattr(torch, n))
+
+
+def readable(*tensors) -> bool:
+    """Whether the memory of these tensors (None: no tensor) holds their values and torch need not see what is done with them: no tracing
+    or compilation, dispatch mode or functional transform, no fake, lazily negated or conjugated tensor, no subclass with a dispatch of its own."""
+    return not torch.compiler.is_compiling() and all(host_statements._readable(t) for t in tensors if t is not None)
+
+
+def torch_watches(*tensors) -> bool:
+    """Whether no kernel may stand for torch operations on these tensors: they are not readable, or a subclass."""
+    return torch.compiler.is_compiling() or not all(_lib.ops().eager(t) for t in tensors if t is not None)
+
+
+def has_tangent(t: torch.Tensor) -> bool:
+    """Whether a forward-mode derivative travels with ``t``."""
+    if torch.compiler.is_compiling() or torch.autograd.forward_ad._current_level < 0:
+        return False
+    return torch.autograd.forward_ad.unpack_dual(t, level=0).tangent is not None
 
 
 def get_dtype_max(dtype: torch.dtype) -> float:

@@ -130,6 +130,24 @@ def test_lazy_negation_and_subclasses(quant, extension, monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("extension", [True, False])
+def test_weights_of_a_class_of_their_own_stay_on_the_kernel(extension, monkeypatch):
+    from flydsl_b200 import row_ops
+    from tests.test_row_ops_gpu import make
+
+    class Weight(torch.nn.Parameter):
+        pass
+
+    if not extension:
+        monkeypatch.setattr(_lib, "_ops", host_statements)
+    x, w = make(16, 256, torch.bfloat16, 9), make(1, 256, torch.bfloat16, 10)[0]
+    want = rmsnorm_quant(x, w)
+    monkeypatch.setattr(row_ops, "_quantised", None)  # not called
+    got = rmsnorm_quant(x, w.as_subclass(Weight))
+    assert type(got[0]) is torch.Tensor and torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
 def test_tangents_are_refused():
     x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
     with fw.dual_level():
