@@ -455,27 +455,72 @@ __global__ void __launch_bounds__(512) rmsnorm_any_kernel(RowParams p) {
 
 // ---- gated activation ---------------------------------------------------------------------------------------------------
 
-// g / (1 + exp(-g)) * u.  exp(-g) = 2^t (1 + ln 2 lo) with t + lo = -g log2(e), lo what the rounding of t left; then g times the reciprocal,
-// which one step of Newton's method makes good to its last place.  From 1 + exp(-g) = 2^126 on (g < -87) the reciprocal is 0, as
-// the value that silu tends to.  Beyond +-88 neither the sum nor the reciprocal changes; the exponent stays there, where 2^t is
-// finite.  NaN comes back with the factor g, and -Inf times 0 is NaN.
-__device__ __forceinline__ float gated(float g, float u) {
-  const float x = fmaxf(fminf(g, 88.0f), -88.0f), t = x * -1.44269504f, lo = fmaf(x, -1.44269504f, -t);
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  const float d = 1.0f + fmaf(e, lo * 0.693147181f, e);
+// g / (1 + exp(-g)) * u.  exp(-x) = 2^t (1 + lo) with t = -x log2(e) rounded and lo = -x - t ln 2, what the roundings of the product and of
+// both constants left; a reciprocal with one step of Newton's method, which makes it good to its last place.
+__device__ __forceinline__ float exp_lo(float x, float t) {
+  constexpr double LN2 = 0.69314718055994530942;
+  constexpr float HIGH = static_cast<float>(LN2), LOW = static_cast<float>(LN2 - static_cast<double>(HIGH));
+  return fmaf(t, -LOW, fmaf(t, -HIGH, -x));
+}
+__device__ __forceinline__ float reciprocal(float d) {
+  float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  if (d < 8.5e37f) r = fmaf(fmaf(-d, r, 1.0f), r, r);
-  return g * r * u;
+  return fmaf(fmaf(-d, r, 1.0f), r, r);
+}
+constexpr float GATE_NEAR = 87.0f;
+// Up to |g| = 87, where neither 1 + exp(-g) nor its reciprocal leaves the range of normal numbers; NaN.
+__device__ __forceinline__ float gated_near(float g, float u) {
+  const float t = g * -1.44269504f;
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return g * reciprocal(1.0f + fmaf(e, exp_lo(g, t), e)) * u;
+}
+// Any g, for g < 0 as g exp(g) / (1 + exp(g)) * u: e = exp(-|g|) keeps the places that fp32 has below 2^-126 and is 0 beyond 104, while
+// u may be large.  -Inf times 0 is NaN.
+__device__ __noinline__ float gated_far(float g, float u) {
+  const float x = fminf(fabsf(g), 105.0f), t = x * -1.44269504f;
+  float e;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t));
+  e = fmaf(e, exp_lo(x, t), e);
+  return g * (g < 0.0f ? e : 1.0f) * reciprocal(1.0f + e) * u;
 }
 
+// All take the form for near gates throughout, and the other one again where one of a thread's gates is far.  That one throughout costs
+// more: 8192 x 28672 bf16 to fp8 268 us in place of 231.
 template <typename T, int N>
 __device__ __forceinline__ void gated_at(const T* xr, int width, int k, float (&v)[N]) {
-  float u[N];
-  unpack(load_raw<T, N>(xr + k), v);
+  float g[N], u[N], top = 0.0f;
+  unpack(load_raw<T, N>(xr + k), g);
   unpack(load_raw<T, N>(xr + width + k), u);
 #pragma unroll
-  for (int j = 0; j < N; ++j) v[j] = gated(v[j], u[j]);
+  for (int j = 0; j < N; ++j) {
+    top = fmaxf(top, fabsf(g[j]));
+    v[j] = gated_near(g[j], u[j]);
+  }
+  if (top > GATE_NEAR) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (fabsf(g[j]) > GATE_NEAR) v[j] = gated_far(g[j], u[j]);
+  }
+}
+
+// Of a row in registers, read once more: the values and their maximum.
+template <typename T, int N, int NV>
+__device__ __forceinline__ void far_gates(const T* xr, int width, int first, int step, float (&v)[NV][N], float& mx) {
+  mx = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int k = first + i * step;
+    if (k >= width) break;
+    float g[N], u[N];
+    unpack(load_raw<T, N>(xr + k), g);
+    unpack(load_raw<T, N>(xr + width + k), u);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (fabsf(g[j]) > GATE_NEAR) v[i][j] = gated_far(g[j], u[j]);
+      mx = max_abs(mx, v[i][j]);
+    }
+  }
 }
 
 // Per-row scale: the row's fp32 values stay in registers between the maximum and the conversion.
@@ -499,7 +544,7 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
       u[i] = load_raw<T, N>(xr + p.width + k);
     }
   }
-  float v[NV][N], mx = 0.0f, none = 0.0f;
+  float v[NV][N], mx = 0.0f, top = 0.0f, none = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if ((i * tpr + tid) * N >= p.width) break;
@@ -508,10 +553,12 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
     unpack(u[i], b);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      v[i][j] = gated(v[i][j], b[j]);
+      top = fmaxf(top, fabsf(v[i][j]));
+      v[i][j] = gated_near(v[i][j], b[j]);
       mx = max_abs(mx, v[i][j]);
     }
   }
+  if (top > GATE_NEAR) far_gates<T, N, NV>(xr, p.width, tid * N, tpr * N, v, mx);
   row_reduce<false, true>(none, mx, wpr, group * wpr, 1 + group, red);
   uint8_t* yr = static_cast<uint8_t*>(p.y) + row * p.width;
   float* scale = static_cast<float*>(p.scale) + row;
@@ -551,7 +598,7 @@ __global__ void __launch_bounds__(1024) silu_row_kernel(RowParams p) {
 // Per-row scale of wide rows, many of them: a row in registers is more than half of an SM's, so there is no second block whose loads
 // could go on while this one reduces, converts and stores.  Here the loads run ahead of all that, over the ends of rows: every thread copies its own
 // vectors into a ring in shared memory and reads them back itself, so that nothing but its own wait stands between the two - no
-// barrier, no flag, no other thread.  us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, 232 here; 250 to 262 with a warp of its own that
+// barrier, no flag, no other thread.  us, 8192 x 28672 bf16 to fp8: 296 with the kernel above, 231 to 236 here; 250 to 262 with a warp of its own that
 // filled the ring by bulk copies (floor 180).
 constexpr int RING_THREADS = 512, RING_WARPS = RING_THREADS / 32;
 constexpr int RING_CHUNK = 16 * RING_THREADS;  // bytes of gate values, and as many of up values: a vector of each per thread
@@ -598,7 +645,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) silu_ring_kernel(RowParams p)
 
   int slot = 0, odd = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    float v[NV][N], mx = 0.0f, none = 0.0f;
+    float v[NV][N], mx = 0.0f, top = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       asm volatile("cp.async.wait_group %0;" ::"n"(RING_SLOTS - 2) : "memory");  // the oldest one is here
@@ -609,13 +656,15 @@ __global__ void __launch_bounds__(RING_THREADS, 1) silu_ring_kernel(RowParams p)
         unpack(load_raw<T, N>(reinterpret_cast<const T*>(at + RING_CHUNK)), u);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          v[i][j] = gated(v[i][j], u[j]);
+          top = fmaxf(top, fabsf(v[i][j]));
+          v[i][j] = gated_near(v[i][j], u[j]);
           mx = max_abs(mx, v[i][j]);
         }
       }
       if (++slot == RING_SLOTS) slot = 0;
       copy_next();  // over the slot that was read one time earlier
     }
+    if (top > GATE_NEAR) far_gates<T, N, NV>(static_cast<const T*>(p.x) + row * p.x_stride, p.width, tid * N, RING_THREADS * N, v, mx);
     row_reduce<false, true>(none, mx, RING_WARPS, 0, 1, reds[odd]);  // nobody writes over it before all are at the next row's barrier
     odd ^= 1;
     uint8_t* yr = static_cast<uint8_t*>(p.y) + row * p.width;
@@ -702,9 +751,10 @@ __global__ void __launch_bounds__(512) silu_any_kernel(RowParams p) {
   }
 }
 
-// No row statistics (MXFP8 blocks, or values of x's type): a thread takes N values wherever they are.
+// No row statistics (MXFP8 blocks, or values of x's type): a thread takes N values wherever they are.  Eight blocks an SM: 8192 x 28672 bf16 216 us
+// (six blocks 230), to MXFP8 300 (320).
 template <typename T, int Q, int N>
-__global__ void __launch_bounds__(256) silu_flat_kernel(RowParams p) {
+__global__ void __launch_bounds__(256, 8) silu_flat_kernel(RowParams p) {
   pdl_wait(p.x, p.y, p.scale);
   pdl_trigger();
   const int per_row = p.width / N;

@@ -45,3 +45,41 @@ def test_zero_rows_without_eps(quant, dtype, k, eps):
     check(y[good], s[good], norm64(x, w, 0.0)[0][good], quant, norm_rel(k))
     y, s, h = rmsnorm_quant(x, torch.zeros_like(w), eps, residual=torch.zeros_like(x), quant_dtype=quant)
     assert not bool(y.float().any()) and bool((s == 1.0).all()) and torch.equal(h, x)
+
+
+# The gated value, by the kernel's steps: 2^t within 2^-22, and rounded once more where it is below 2^-126; its correction, 1 + exp and the
+# products round once each, the reciprocal is good to its last place: 11 units of 2^-24, and the next power of two is SILU_REL.  Below 2^-126 an
+# exponential is off by up to two steps of 2^-149: |g u| times that.  A result below 2^-126 is off by a step itself.
+def gated_bound(x, v):
+    g, u = x.double().chunk(2, dim=-1)
+    return SILU_REL * v.abs() + (g * u).abs() * 2.0**-148 + 2.0**-149
+
+
+@pytest.mark.parametrize("lo,hi", [(-1.0, 1.0), (-20.0, 20.0), (-87.0, -60.0), (-89.0, -86.0), (-104.0, -88.0), (-300.0, -100.0), (60.0, 300.0)])
+@pytest.mark.parametrize("up", [1.0, 1e38, 1e-6])
+def test_gated_values_hold_fp32(lo, hi, up):
+    """Without a floor: between -88 and -104 exp(g) is below 2^-126, but a product with a large `up` is not."""
+    k = 65536
+    g = torch.linspace(lo, hi, k, device="cuda")
+    u = torch.full_like(g, up) * torch.where(torch.arange(k, device="cuda") % 3 == 0, -1.0, 0.75)
+    x = torch.cat([g, u])[None]
+    y, none = silu_mul_quant(x, quant_dtype=None)
+    v = silu64(x)
+    keep = v.abs() < 3.4e38
+    assert none is None and bool(torch.isinf(y[~keep & (v.abs() > 3.41e38)]).all())
+    err = (y.double() - v).abs()
+    assert bool((err <= gated_bound(x, v))[keep].all()), float((err / gated_bound(x, v))[keep].max())
+
+
+@pytest.mark.parametrize("inter,rows", [(96, 5), (1003, 5), (5120, 300)])
+@pytest.mark.parametrize("quant", [FP8, torch.int8, "mxfp8"], ids=["fp8", "int8", "mxfp8"])
+def test_rows_of_gates_far_below_zero(quant, inter, rows):
+    """What such gates leave is all that a row has."""
+    if quant == "mxfp8":
+        inter = -(-inter // 32) * 32
+    g = torch.Generator(device="cuda").manual_seed(42)
+    gate = -87.0 - 3.0 * torch.rand(rows, inter, generator=g, device="cuda")
+    x = torch.cat([gate, 1e35 * torch.randn(rows, inter, generator=g, device="cuda")], dim=-1)
+    y, s = silu_mul_quant(x, quant_dtype=quant)
+    # exp(g) is at least 2^-130 there: two steps of 2^-149 are 2^-18 of it
+    check(y, s, silu64(x), quant, SILU_REL + 2.0**-18)
