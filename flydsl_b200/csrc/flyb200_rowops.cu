@@ -261,6 +261,23 @@ __device__ __forceinline__ void store_mx(uint8_t* y, uint8_t* scale, int k, bool
 
 // ---- norm ---------------------------------------------------------------------------------------------------------------
 
+// h w f, multiplied in the order that stays in range: h w may be infinite where h f w is not, and a very large f (no eps, small rows)
+// may bring back what h w has lost below 2^-126.  Up to this f that is at most 2^-126 of the value.
+constexpr float LARGE_F = 16777216.0f;
+__device__ __forceinline__ float normed(float h, float w, float f) {
+  const float v = h * w;
+  return fabsf(v) < INFINITY && f <= LARGE_F ? v * f : h * f * w;
+}
+// N values from what the thread has read or written before.
+template <typename T, int N>
+__device__ __forceinline__ void normed_at(const RowParams& p, const T* row, int k, float f, float (&v)[N]) {
+  float h[N], w[N];
+  unpack(load_raw<T, N>(row + k), h);
+  load_weight<T, N>(p, k, w);
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = normed(h[j], w[j], f);
+}
+
 // Sum of squares and maximum of |h w| of N elements.
 template <bool MAX, int N>
 __device__ __forceinline__ void norm_stats(const float (&h)[N], const float (&w)[N], float& sum, float& mx) {
@@ -317,7 +334,7 @@ __global__ void __launch_bounds__(NV == 8 ? 512 : 1024) rmsnorm_row_kernel(RowPa
     for (int j = 0; j < N; ++j) {
       sum = fmaf(v[i][j], v[i][j], sum);
       v[i][j] *= w[j];
-      if constexpr (ROWQ) mx = max_abs(mx, v[i][j]);
+      mx = max_abs(mx, v[i][j]);  // without codes per row, the thread's own
     }
   }
   row_reduce<true, ROWQ>(sum, mx, wpr, group * wpr, 1 + group, red);
@@ -338,39 +355,48 @@ __global__ void __launch_bounds__(NV == 8 ? 512 : 1024) rmsnorm_row_kernel(RowPa
         store_codes<Q, N>(yr + k, v[i]);
       }
     } else {  // the same branch in all threads of the row
-      float amax = 0.0f, none = 0.0f;
+      const T* again = p.r ? hr : xr;
+      float far[N], amax = 0.0f, none = 0.0f;
+#pragma unroll 1
+      for (int k = tid * N; k < p.width; k += tpr * N) {
+        normed_at(p, again, k, f, far);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if ((i * tpr + tid) * N >= p.width) break;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          v[i][j] *= f;
-          amax = fmaxf(amax, fabsf(scrub(v[i][j], QMAX_OF<Q>)));
-        }
+        for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(scrub(far[j], QMAX_OF<Q>)));
       }
       if (wpr > 1) named_bar_sync(1 + group, tpr);  // `red` is read above
       row_reduce<false, true>(none, amax, wpr, group * wpr, 1 + group, red);
       float s = __fmul_rn(amax, 1.0f / QMAX_OF<Q>);
       if (s == 0.0f) s = 1.0f;
       if (tid == 0) *scale = s;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int k = (i * tpr + tid) * N;
-        if (k >= p.width) break;
-        store_codes_divided<Q, N>(yr + k, v[i], s);
+#pragma unroll 1
+      for (int k = tid * N; k < p.width; k += tpr * N) {
+        normed_at(p, again, k, f, far);
+        store_codes_divided<Q, N>(yr + k, far, s);
       }
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = (i * tpr + tid) * N;
+    auto store = [&](int k, const float (&u)[N]) {
       const bool in = k < p.width;
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[i][j] *= f;
       if constexpr (Q == Q_MXFP8) {
-        store_mx<N>(static_cast<uint8_t*>(p.y) + row * p.width, static_cast<uint8_t*>(p.scale) + row * (p.width / 32), k, in, v[i]);
+        store_mx<N>(static_cast<uint8_t*>(p.y) + row * p.width, static_cast<uint8_t*>(p.scale) + row * (p.width / 32), k, in, u);
       } else if (in) {
-        store_raw<T, N>(static_cast<T*>(p.y) + row * p.width + k, pack<T, N>(v[i]));
+        store_raw<T, N>(static_cast<T*>(p.y) + row * p.width + k, pack<T, N>(u));
+      }
+    };
+    if (__all_sync(0xffffffffu, mx < INFINITY && f <= LARGE_F)) {  // a warp's lanes meet in store_mx
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i][j] *= f;
+        store((i * tpr + tid) * N, v[i]);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < NV; ++i) {
+        const int k = (i * tpr + tid) * N;
+        float u[N] = {};
+        if (k < p.width) normed_at(p, p.r ? hr : xr, k, f, u);
+        store(k, u);
       }
     }
   }
@@ -417,11 +443,10 @@ __global__ void __launch_bounds__(512) rmsnorm_any_kernel(RowParams p) {
       } else {
         float amax = 0.0f, none = 0.0f;
         for (int k = threadIdx.x * N; k < p.width; k += step) {
-          float h[N], w[N];
-          unpack(load_raw<T, N>(xr + k), h);
-          load_weight<T, N>(p, k, w);
+          float v[N];
+          normed_at(p, xr, k, f, v);
 #pragma unroll
-          for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(scrub(h[j] * w[j] * f, QMAX_OF<Q>)));
+          for (int j = 0; j < N; ++j) amax = fmaxf(amax, fabsf(scrub(v[j], QMAX_OF<Q>)));
         }
         row_reduce<false, true>(none, amax, wpr, 0, 1, red);
         __syncthreads();
@@ -439,7 +464,7 @@ __global__ void __launch_bounds__(512) rmsnorm_any_kernel(RowParams p) {
         unpack(load_raw<T, N>(xr + k), h);
         load_weight<T, N>(p, k, w);
 #pragma unroll
-        for (int j = 0; j < N; ++j) h[j] = ROWQ && !s.divide ? in_units<Q>(h[j] * w[j], s) : h[j] * w[j] * f;
+        for (int j = 0; j < N; ++j) h[j] = ROWQ && !s.divide ? in_units<Q>(h[j] * w[j], s) : normed(h[j], w[j], f);
       }
       if constexpr (ROWQ) {
         uint8_t* y = static_cast<uint8_t*>(p.y) + row * p.width + k;

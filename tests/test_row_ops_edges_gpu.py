@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from flydsl_b200 import rmsnorm_quant, silu_mul_quant
-from tests.test_row_ops_gpu import FP8, SILU_REL, TYPES, check, make, norm64, norm_rel, silu64
+from tests.test_row_ops_gpu import FP8, IDS, QUANTS, SILU_REL, TYPES, check, half_step, make, norm64, norm_rel, silu64
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,34 @@ def test_rows_of_gates_far_below_zero(quant, inter, rows):
     y, s = silu_mul_quant(x, quant_dtype=quant)
     # exp(g) is at least 2^-130 there: two steps of 2^-149 are 2^-18 of it
     check(y, s, silu64(x), quant, SILU_REL + 2.0**-18)
+
+
+@pytest.mark.parametrize("k", [4096, 1003, 40000])
+@pytest.mark.parametrize("dtype,size,weight,eps", [(torch.float32, 1e15, 1e25, 1e-6), (torch.bfloat16, 1e15, 1e25, 1e-6), (torch.float16, 100.0, 1e38, 1e-6),
+                                                   (torch.float32, 1e-15, 1e-27, 0.0), (torch.bfloat16, 1e-15, 1e-27, 0.0)],
+                         ids=["large32", "largebf16", "largefp16", "small32", "smallbf16"])
+@pytest.mark.parametrize("quant", QUANTS, ids=IDS)
+def test_norm_where_input_times_weight_leaves_fp32(quant, dtype, size, weight, eps, k):
+    """h w is out of range while h w / rms(h) is not."""
+    if quant == "mxfp8":
+        k = -(-k // 32) * 32
+    if quant is None and dtype == torch.float16:
+        dtype = torch.bfloat16  # values of 1e38 are none of fp16
+    x = (torch.randn(6, k, generator=torch.Generator(device="cuda").manual_seed(43), device="cuda") * size).to(dtype)
+    w = (1.0 + torch.rand(k, generator=torch.Generator(device="cuda").manual_seed(44), device="cuda")) * weight / 4
+    w = w if dtype == torch.float16 else w.to(dtype)
+    x[3] *= 1e-3
+    r = (x * 0.25).to(dtype)
+    for residual in (None, r):
+        y, s, h = rmsnorm_quant(x, w, eps, residual=residual, quant_dtype=quant)
+        v, h64 = norm64(x, w, eps, residual)
+        assert residual is None or torch.equal(h, h64)
+        if quant != "mxfp8":
+            check(y, s, v, quant, norm_rel(k))
+            continue
+        # the quantiser divides by at least 1e-30, also where the scale byte says less
+        b, unit = v.reshape(6, -1, 32), torch.pow(2.0, s.double() - 127)[..., None]
+        q = (b / unit.clamp_min(1e-30)).clamp(-448, 448)
+        top = b.abs().amax(-1, keepdim=True)
+        assert bool((top <= 448 * 1.5 * unit * (1 + 2**-16)).all() and (top >= 448 * 0.75 * unit * (1 - 2**-16)).all())
+        assert bool(((y.reshape(b.shape).double() - q).abs() <= half_step(q, FP8) + norm_rel(k) * q.abs()).all())
