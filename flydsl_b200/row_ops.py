@@ -92,15 +92,23 @@ def _outputs(x: torch.Tensor, width: int, quant: int):
     return y, torch.empty(*shape, 1, dtype=torch.float32, device=x.device)
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges of two tensors meet."""
+def _span(t: torch.Tensor, rows: int, stride: int) -> tuple[int, int, int, int]:
+    """(address, rows, distance, width) in bytes; one row has no distance."""
+    e = t.element_size()
+    return t.data_ptr(), rows, stride * e if rows > 1 else 0, t.shape[-1] * e
 
-    def span(t):
-        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else -1
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+def _share(a, b) -> bool:
+    """Whether two runs of rows (`_span`) share memory.  At one distance, or where one is a single row, that is decided row by row: other columns
+    of one buffer are apart.  At two distances the address ranges decide."""
+    (a0, ra, sa, wa), (b0, rb, sb, wb) = a, b
+    if ra == 0 or rb == 0 or b0 >= a0 + (ra - 1) * sa + wa or a0 >= b0 + (rb - 1) * sb + wb:
+        return False
+    step = sa or sb
+    if not step or (sa and sb and sa != sb):
+        return True
+    d = (b0 - a0) % step  # from a row of a to the next start of a row of b
+    return d < wa or d + wb > step
 
 
 def _quantised(v: torch.Tensor, dtype: torch.dtype, quant: int):
@@ -153,11 +161,13 @@ def rmsnorm_quant(x, weight, eps=1e-6, *, residual=None, quant_dtype=torch.float
         r_stride = _rows("residual", residual, x)[1]
         h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual_out is None else residual_out
         h_stride = _rows("residual_out", h, x)[1]
-        for name, t in (("x", x), ("residual", residual)) if not watched else ():
-            if residual_out is not None and _overlap(h, t) and (h.data_ptr() != t.data_ptr() or h.stride() != t.stride()):
-                raise ValueError(f"residual_out overlaps {name} without being the same tensor")
-        if residual_out is not None and not watched and _overlap(h, weight):
-            raise ValueError("residual_out overlaps weight")
+        if residual_out is not None and not watched:
+            out = _span(h, rows, h_stride)
+            for name, span in (("x", _span(x, rows, stride)), ("residual", _span(residual, rows, r_stride))):
+                if span != out and _share(out, span):
+                    raise ValueError(f"residual_out overlaps {name} without being the same tensor")
+            if _share(out, _span(weight, 1, k)):
+                raise ValueError("residual_out overlaps weight")
     y, scale = _outputs(x, k, quant)
     if rows == 0:
         return y, scale, h

@@ -114,3 +114,24 @@ def test_norm_where_input_times_weight_leaves_fp32(quant, dtype, size, weight, e
         top = b.abs().amax(-1, keepdim=True)
         assert bool((top <= 448 * 1.5 * unit * (1 + 2**-16)).all() and (top >= 448 * 0.75 * unit * (1 - 2**-16)).all())
         assert bool(((y.reshape(b.shape).double() - q).abs() <= half_step(q, FP8) + norm_rel(k) * q.abs()).all())
+
+
+def test_sums_beside_the_inputs_in_one_buffer():
+    """residual_out in other columns of the buffer that x lies in: their address ranges cross, their elements do not."""
+    k = 256
+    buf, r = make(20, 3 * k, torch.bfloat16, 45), make(20, k, torch.bfloat16, 46)
+    w = make(1, k, torch.bfloat16, 47)[0]
+    x = buf[:, :k]
+    want = rmsnorm_quant(x.clone(), w, residual=r)
+    kept = buf.clone()
+    y, s, h = rmsnorm_quant(x, w, residual=r, residual_out=buf[:, 2 * k :])
+    assert torch.equal(h, want[2]) and torch.equal(y.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s, want[1])
+    assert torch.equal(buf[:, : 2 * k], kept[:, : 2 * k]) and h.data_ptr() == buf[:, 2 * k :].data_ptr()
+    for at in (1, k - 1):
+        with pytest.raises(ValueError, match="overlaps x"):
+            rmsnorm_quant(x, w, residual=r, residual_out=buf[:, at : at + k])
+    # one row: its distance to the next one says nothing
+    one = buf[:1, :k]
+    want = rmsnorm_quant(one.clone(), w, residual=r[:1])
+    same = one.as_strided((1, k), (7 * k, 1))
+    assert torch.equal(rmsnorm_quant(one, w, residual=r[:1], residual_out=same)[2], want[2]) and torch.equal(one, want[2])
