@@ -77,8 +77,9 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[WORDS]) {
 //
 // The accumulators start at the bits of 1.5 * 2^23, so that the sum D of a column comes out as the number 1.5 * 2^23 + D.
 // With its fp32 companions of a group, f = 2^e and f sum(X) of every limb, a column adds
-// scale * (f D - zero f sum(X)) to the result in fp32; the limbs are put together at the end.  f is kept as a quarter and the scale
-// as its fourfold, so that 1.5 * 2^23 f stays in range for the largest bf16 numbers.
+// scale * (f D - zero f sum(X)) to the result in fp32; the limbs are put together at the end.  f is kept as a quarter, so that
+// 1.5 * 2^23 f stays in range for the largest bf16 numbers, and the result is taken times 4.  For the smallest ones f is below 2^-126; it and
+// its products with integers below 2^24 are exact there.
 constexpr uint32_t INT_BITS = 0x4B400000u;
 constexpr float INT_BASE = 12582912.0f;
 
@@ -246,14 +247,16 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
 #pragma unroll
     for (int o = 1; o < G / 8; o <<= 1) top = max(top, __shfl_xor_sync(lanes, top, o));
     const bool finite = top < 0x7F800000u;
-    const uint32_t e = max(top >> 23, 24u);                     // 2^(e - 127) <= max < 2^(e - 126)
-    const float up = __uint_as_float((275u - e) << 23);         // 2^(148 - e): |v up| < 2^22
-    const float f = finite ? __uint_as_float((e - 23u) << 23) : __uint_as_float(0x7FFFFFFFu);
+    const uint32_t e = max(top >> 23, 1u);                      // max < 2^(e - 126); 2^(e - 127) <= max but for numbers below 2^-126
+    const uint32_t few = e < 24u ? 24u - e : 0u;                // 2^(148 - e) in two factors where it is no fp32 number
+    const float lift = __uint_as_float((127u + few) << 23);
+    const float up = __uint_as_float((275u - e - few) << 23);   // |v lift up| < 2^22
+    const float f = !finite ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(e > 23u ? (e - 23u) << 23 : 1u << (e - 1u));  // 2^(e - 150)
     uint32_t u[8];
     int sum[3] = {0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t x = finite ? __float_as_uint(fmaf(v[j], up, INT_BASE)) - INT_BITS : 0u;
+      const uint32_t x = finite ? __float_as_uint(fmaf(v[j] * lift, up, INT_BASE)) - INT_BITS : 0u;
       u[j] = (x + 0x808080u) ^ 0x808080u;  // bytes 0, 1, 2: the limbs
     }
     uint2 limb[3];
@@ -309,7 +312,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
       float scale[LOADS], zero[LOADS];
 #pragma unroll
       for (int u = 0; u < LOADS; ++u) {
-        scale[u] = 4.0f * W4<T>::value(next_scale[u]);
+        scale[u] = W4<T>::value(next_scale[u]);
         zero[u] = -static_cast<float>(next_zero[u] & 15);
       }
       load_scales();
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
         const int n = 16 * r + 8 * h + g;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float v = c & 1 ? 65536.0f * acc[r][t][2 * h] : fmaf(256.0f, acc[r][t][2 * h + 1], acc[r][t][2 * h]);
+          float v = c & 1 ? 262144.0f * acc[r][t][2 * h] : 4.0f * fmaf(256.0f, acc[r][t][2 * h + 1], acc[r][t][2 * h]);
           v += __shfl_xor_sync(0xffffffffu, v, 1);
           const int m = 2 * t + (c >> 1);
           if ((c & 1) == 0 && m < p.M) part[m * S::R + n] = v;

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
     for (int h = 0; h < halves; ++h) {
       float scale[GROUPS];
 #pragma unroll
-      for (int j = 0; j < GROUPS; ++j) scale[j] = (2 * s0 + h) * GROUPS + j < n_groups ? W4<T>::UNIT * W4<T>::value(next[j]) : 0.0f;
+      for (int j = 0; j < GROUPS; ++j) scale[j] = (2 * s0 + h) * GROUPS + j < n_groups ? W4<T>::value(next[j]) : 0.0f;
       if (h + 1 < halves) load_scales(h + 1);
       if (!wait_of<NT>(done + 8 * slot, slot_phase, abort_flag)) {
         if (lane == 0) report_failure(p.status, ST_TIMEOUT, abort_flag);
@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(Wide<NT, G>::THREADS, 1)
 
   // ---- the result: of a block by itself from registers, of a cluster through shared memory, added up in the order of its blocks ----
   auto store = [&](int m, int n, float v) {
+    v *= W4<T>::UNIT;
     if (p.epilogue != EPI_NONE) v = w4_activation(v + W4<T>::value(static_cast<const unsigned short*>(p.bias)[n]), p.epilogue);
     static_cast<T*>(p.c)[static_cast<size_t>(m) * p.N + n] = W4<T>::round(v);
   };

@@ -1,0 +1,22 @@
+"""The products on 4-bit weights at the ends of what their types and arguments allow."""
+
+import pytest
+import torch
+
+from flydsl_b200 import compile_w4a16_gemv
+from tests.test_w4_gemv_gpu import check, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("m", [1, 4, 5, 40])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("size,scale", [(2.0**-90, 2.0**118), (2.0**-90, 2.0**126), (2.0**-110, 2.0**90), (2.0**-118, 2.0**100), (2.0**-124, 2.0**110)])
+def test_scales_and_activations_at_opposite_ends(m, group, size, scale):
+    """Products in range of large scales and small activations; bf16 as the range of fp16 has neither."""
+    a, q, s, z, _ = make(m, 64, 512, group, "bf16", True, 11)
+    x = ((1.0 + a.float().abs().clamp(max=0.9)) * size * torch.sign(a.float() + 1e-3)).to(torch.bfloat16)
+    t = torch.full_like(s, scale)
+    c = torch.empty(m, 64, dtype=torch.bfloat16, device="cuda")
+    compile_w4a16_gemv(N=64, K=512, group_size=group, zero_points=True)(c, x, q, t, z, None, m, 64)
+    check(c, x, q, t, z, None, group)
