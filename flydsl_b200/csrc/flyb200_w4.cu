@@ -552,13 +552,13 @@ extern "C" int flyb200_gemv_w4a16(void* c, const void* a, const void* q, const v
   if (dtype != FLYB200_DT_FP16 && dtype != FLYB200_DT_BF16) return FLYB200_E_BAD_ARG;
   if (epilogue < FLYB200_EPI_NONE || epilogue > FLYB200_EPI_BIAS_GELU || (epilogue != FLYB200_EPI_NONE && !bias)) return FLYB200_E_BAD_ARG;
   if (group != 32 && group != 64 && group != 128) return FLYB200_E_BAD_ARG;
-  if (K % group != 0 || N > (1 << 27) || K > (1 << 26) || M > 8 * 65535) return FLYB200_E_UNSUPPORTED;
+  if (K % group != 0 || N > (1 << 27) || K > (1 << 26)) return FLYB200_E_UNSUPPORTED;
   auto multiple = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
   if (!multiple(a, 16) || !multiple(q, 16) || !multiple(c, 2) || !multiple(scale, 2) || !multiple(bias, 2)) return FLYB200_E_BAD_ALIGN;
   if (M == 0) return FLYB200_OK;
   const bool fp16 = dtype == FLYB200_DT_FP16;
-  for (int m = 0; m < M; m += WIDE_TOKENS) {
-    const int tokens = M - m < WIDE_TOKENS ? M - m : WIDE_TOKENS;
+  for (long long m = 0; m < M; m += WIDE_TOKENS) {
+    const int tokens = static_cast<int>(M - m < WIDE_TOKENS ? M - m : WIDE_TOKENS);
     char* cm = static_cast<char*>(c) + static_cast<size_t>(m) * N * 2;
     const char* am = static_cast<const char*>(a) + static_cast<size_t>(m) * K * 2;
     W4Params p = {cm, am, static_cast<const uint8_t*>(q), scale, static_cast<const uint8_t*>(zero), bias, tokens, N, K, epilogue};

@@ -242,7 +242,8 @@ int flyb200_silu_mul_quant(void* y, void* scale, const void* x, int rows, int in
  *   zero     [N, K / group] bytes 0..15, or NULL: 8 everywhere (codes are then signed numbers plus 8)
  *   bias     [N] of the type of a; NULL when epilogue == FLYB200_EPI_NONE
  * Code minus zero point is an exact number in the multiply; sums over a group are fp32 and the scale multiplies them in fp32.
- * Requirements: group 32, 64 or 128, K a multiple of it; a and q 16-byte aligned. */
+ * Requirements: group 32, 64 or 128, K a multiple of it; a and q 16-byte aligned; N up to 2^27, K up to 2^26; c apart from the inputs.
+ * Any M: blocks of 64 tokens that each read the weights. */
 int flyb200_gemv_w4a16(void* c, const void* a, const void* q, const void* scale, const void* zero, const void* bias, int M, int N,
                        int K, int group, int dtype, int epilogue, void* stream);
 

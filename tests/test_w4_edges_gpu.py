@@ -20,3 +20,13 @@ def test_scales_and_activations_at_opposite_ends(m, group, size, scale):
     c = torch.empty(m, 64, dtype=torch.bfloat16, device="cuda")
     compile_w4a16_gemv(N=64, K=512, group_size=group, zero_points=True)(c, x, q, t, z, None, m, 64)
     check(c, x, q, t, z, None, group)
+
+
+def test_more_tokens_than_a_grid_has_rows():
+    """Any number of tokens, in blocks of 64; the last one of 5."""
+    m, n, k = 8 * 65535 + 13, 1, 32
+    a, q, s, z, _ = make(m, n, k, 32, "bf16", True, 12)
+    c = torch.full((m + 1, n), -77.0, dtype=torch.bfloat16, device="cuda")
+    compile_w4a16_gemv(N=n, K=k, group_size=32, zero_points=True)(c, a, q, s, z, None, m, n)
+    assert bool((c[m:] == -77.0).all())
+    check(c[:m], a, q, s, z, None, 32)
