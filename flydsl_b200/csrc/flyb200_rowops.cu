@@ -292,7 +292,7 @@ __device__ __forceinline__ void norm_stats(const float (&h)[N], const float (&w)
 // residual to fp8: 212 us with the sums as they were read and read twice, 185 with h w in fp32 between the passes and packed additions, 170 with
 // two vectors a thread in place of four (64 registers and spills); floor 144.
 template <typename T, int Q, int NV>
-__global__ void __launch_bounds__(NV == 8 ? 512 : 1024) rmsnorm_row_kernel(RowParams p) {
+__global__ void __launch_bounds__(1024) rmsnorm_row_kernel(RowParams p) {
   constexpr int N = VEC_OF<T>;
   constexpr bool ROWQ = Q == Q_FP8 || Q == Q_INT8;
   __shared__ float red[64];
@@ -804,6 +804,8 @@ __global__ void __launch_bounds__(256, 8) silu_flat_kernel(RowParams p) {
     if (_e != cudaSuccess) return host::record_cuda_error(_e, #expr);   \
   } while (0)
 
+constexpr int SMS = 148;  // that the shapes of launches are meant for
+
 bool multiple(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // Warps that share a row of `vecs` vectors, at most `most_vecs` per thread: as few as that allows, more while the rows
@@ -812,7 +814,7 @@ int warps_per_row(int rows, int vecs, int most_vecs, int most_warps) {
   int wpr = 1;
   while (wpr < most_warps && vecs > 32 * wpr * most_vecs) wpr *= 2;
   if (vecs > 32 * wpr * most_vecs) return 0;
-  while (wpr < most_warps && vecs > 32 * wpr && static_cast<long long>(rows) * wpr < 2LL * 148 * 8) wpr *= 2;
+  while (wpr < most_warps && vecs > 32 * wpr && static_cast<long long>(rows) * wpr < 2LL * SMS * 8) wpr *= 2;
   return wpr;
 }
 int threads_of(int wpr) { return 32 * (wpr < 8 ? 8 : wpr); }
@@ -820,28 +822,26 @@ unsigned blocks_of(int rows, int wpr) {
   const int per = wpr < 8 ? 8 / wpr : 1;
   return static_cast<unsigned>((static_cast<long long>(rows) + per - 1) / per);
 }
-constexpr int ANY_BLOCKS = 148 * 4;
+constexpr int ANY_BLOCKS = SMS * 4;
 
 template <typename T, int Q>
 cudaError_t launch_norm(RowParams p, bool vectors, cudaStream_t s) {
   constexpr int N = VEC_OF<T>;
   const int vecs = p.width / N;
-  int wpr = vectors ? warps_per_row(p.rows, vecs, N == 8 ? 2 : 4, 32) : 0, nv = 0;
+  int wpr = vectors ? warps_per_row(p.rows, vecs, N == 8 ? 2 : 4, 32) : 0;
   if (vectors && !wpr) wpr = warps_per_row(p.rows, vecs, 4, 32);
-  if (wpr) nv = (vecs + 32 * wpr - 1) / (32 * wpr);
-  else if (vectors && (wpr = warps_per_row(p.rows, vecs, 8, 16)) != 0) nv = 8;
-  if (!nv) {
+  if (!wpr) {
     const dim3 grid(p.rows < ANY_BLOCKS ? p.rows : ANY_BLOCKS);
     return vectors ? host::launch_dependent(rmsnorm_any_kernel<T, Q, N>, grid, 512, 0, s, p)
                    : host::launch_dependent(rmsnorm_any_kernel<T, Q, 1>, grid, 512, 0, s, p);
   }
+  const int nv = (vecs + 32 * wpr - 1) / (32 * wpr);
   p.warps_per_row = wpr;
   const dim3 grid(blocks_of(p.rows, wpr));
   const int t = threads_of(wpr);
   return nv == 1   ? host::launch_dependent(rmsnorm_row_kernel<T, Q, 1>, grid, t, 0, s, p)
          : nv == 2 ? host::launch_dependent(rmsnorm_row_kernel<T, Q, 2>, grid, t, 0, s, p)
-         : nv <= 4 ? host::launch_dependent(rmsnorm_row_kernel<T, Q, 4>, grid, t, 0, s, p)
-                   : host::launch_dependent(rmsnorm_row_kernel<T, Q, 8>, grid, t, 0, s, p);
+                   : host::launch_dependent(rmsnorm_row_kernel<T, Q, 4>, grid, t, 0, s, p);
 }
 
 // Vectors of a row from which on the ring is taken.
@@ -873,7 +873,7 @@ cudaError_t launch_silu(RowParams p, bool vectors, cudaStream_t s) {
                    : host::launch_dependent(silu_flat_kernel<T, Q, 1>, dim3(static_cast<unsigned>(blocks)), 256, 0, s, p);
   } else {
     const int vecs = p.width / N;
-    if (vectors && vecs > RING_FROM && vecs <= 8 * RING_THREADS && p.rows > 148) {
+    if (vectors && vecs > RING_FROM && vecs <= 8 * RING_THREADS && p.rows > SMS) {
       const int nv = (vecs + RING_THREADS - 1) / RING_THREADS;
       return nv <= 3   ? launch_silu_ring<T, Q, 3>(p, s)
              : nv == 4 ? launch_silu_ring<T, Q, 4>(p, s)
