@@ -48,15 +48,10 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
 template <int WORDS>
 __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[WORDS]) {
   if constexpr (WORDS == 4) {
-    const uint4 v = lds128(a);
+    const uint4 v = ld_smem_v4(a);
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   } else if constexpr (WORDS == 2) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
@@ -83,11 +78,12 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[WORDS]) {
 constexpr uint32_t INT_BITS = 0x4B400000u;
 constexpr float INT_BASE = 12582912.0f;
 
-template <int MT, int NT>
+constexpr int MT = 2;  // tiles of 16 rows of weights in a warp
+
 struct IntShape {
   static constexpr int R = 16 * MT;
   static constexpr int STAGE = 1024 * MT;
-  static constexpr int STAGES = MT == 1 ? 5 : 4;
+  static constexpr int STAGES = 4;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int SMEM = 227 * 1024;
   // of `steps` steps of M tokens: three bytes an activation, four floats a token and group
@@ -120,9 +116,9 @@ __device__ __forceinline__ int chunk_place(int chunk, int col) {
 //
 // Chunks of 16 bytes of codes are stored with their number XOR-ed by the row so that the reads of a warp meet no bank twice.
 // Rows behind the last weight row are read in place of ones that do not exist; what comes out is not stored.
-template <typename T, int G, int MT, int NT>
+template <typename T, int G, int NT>
 __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) {
-  using S = IntShape<MT, NT>;
+  using S = IntShape;
   constexpr int GROUPS = CHUNK / G;  // of a step
   constexpr int WORDS = G / 32;      // words of a lane per row and group
   constexpr int SLOTS = GROUPS * 2 * MT;  // scales that a lane needs of a step: group j, rows 16 r + 8 h + g at slot (j MT + r) 2 + h
@@ -328,7 +324,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
           } else {
 #pragma unroll
             for (int i = 0; i < WORDS; i += 2) {
-              const uint4 v = lds128(x_chunk[t][WORDS == 4 ? i / 2 : j] + x_at);
+              const uint4 v = ld_smem_v4(x_chunk[t][WORDS == 4 ? i / 2 : j] + x_at);
               x[t][i][0] = v.x, x[t][i][1] = v.y, x[t][i + 1][0] = v.z, x[t][i + 1][1] = v.w;
             }
           }
@@ -410,11 +406,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) gemv_w4_int_kernel(W4Params p) 
       if (p.split > 1) {
         const uint32_t at = smem_u32(from);
         v = 0.0f;
-        for (int k = 0; k < p.split; ++k) {
-          float o;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(map_to_cta(at, k)) : "memory");
-          v += o;
-        }
+        for (int k = 0; k < p.split; ++k) v += __uint_as_float(ld_dsmem(map_to_cta(at, k)));
       } else {
         v = from[0];
         for (int w = 1; w < p.wk; ++w) v += from[w * p.M * S::R];
@@ -466,10 +458,10 @@ cudaError_t clusters_at_once(Kernel kernel, int split, int sms, int smem, int* o
   return cudaSuccess;
 }
 
-template <typename T, int G, int MT, int NT>
+template <typename T, int G, int NT>
 cudaError_t launch_int(W4Params p, int split, cudaStream_t s) {
-  using S = IntShape<MT, NT>;
-  auto kernel = gemv_w4_int_kernel<T, G, MT, NT>;
+  using S = IntShape;
+  auto kernel = gemv_w4_int_kernel<T, G, NT>;
   static std::atomic<uint64_t> done{0};
   int dev = 0, sms = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return e;
@@ -517,9 +509,9 @@ cudaError_t launch_int(W4Params p, int split, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 // Blocks of a cluster: as few as leave room for the activations and the sums of a tile.  0: none do.
-template <typename T, int G, int MT, int NT>
+template <typename T, int G, int NT>
 int split_of(const W4Params& p) {
-  using S = IntShape<MT, NT>;
+  using S = IntShape;
   const int steps = (p.K + CHUNK - 1) / CHUNK;
   for (int split = 1; split <= 8; split *= 2) {
     const int part = (steps + split - 1) / split;
@@ -528,16 +520,16 @@ int split_of(const W4Params& p) {
   }
   return 0;
 }
-template <typename T, int G, int MT, int NT>
+template <typename T, int G, int NT>
 bool try_int(const W4Params& p, cudaStream_t s, cudaError_t& e) {
-  const int split = split_of<T, G, MT, NT>(p);
-  if (split) e = launch_int<T, G, MT, NT>(p, split, s);
+  const int split = split_of<T, G, NT>(p);
+  if (split) e = launch_int<T, G, NT>(p, split, s);
   return split != 0;
 }
 // False where the activations of so many inputs do not fit.
 template <typename T, int G>
 bool few_tokens(const W4Params& p, cudaStream_t s, cudaError_t& e) {
-  return p.M <= 2 ? try_int<T, G, 2, 1>(p, s, e) : try_int<T, G, 2, 2>(p, s, e);
+  return p.M <= 2 ? try_int<T, G, 1>(p, s, e) : try_int<T, G, 2>(p, s, e);
 }
 template <typename T>
 bool few_tokens(const W4Params& p, int group, cudaStream_t s, cudaError_t& e) {

@@ -4,7 +4,8 @@
 
 namespace flyb200 {
 
-// A code becomes the 16-bit number MAGIC + code by putting it into the last places of MAGIC's mantissa; less() then takes the zero
+// The usual way to decode small integers without a conversion: a code becomes the 16-bit number MAGIC + code by putting it into the last
+// places of MAGIC's mantissa; less() then takes the zero
 // point off, given as the bits ZERO + zero point, exactly.  bf16: the result is q - z times 2^-12, so that the sum of a
 // group stays in the range of fp32 whatever the activations are; UNIT takes it back from the result, where a scale times UNIT need not be
 // in range.
