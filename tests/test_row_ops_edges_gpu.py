@@ -135,3 +135,26 @@ def test_sums_beside_the_inputs_in_one_buffer():
     want = rmsnorm_quant(one.clone(), w, residual=r[:1])
     same = one.as_strided((1, k), (7 * k, 1))
     assert torch.equal(rmsnorm_quant(one, w, residual=r[:1], residual_out=same)[2], want[2]) and torch.equal(one, want[2])
+
+
+@pytest.mark.parametrize("k", [4096, 4095])
+def test_rows_past_four_gigabytes(k):
+    """Inputs beyond 2^32 bytes and outputs beyond 2^31 elements, of rows that repeat after 61: an offset that wraps meets another row.  Whole
+    vectors, and odd rows.  Other numbers of rows sum in another order."""
+    rows = (1 << 31) // k + 70
+    tail = torch.arange(rows - 122, rows, device="cuda") % 61
+    w = make(1, k, torch.bfloat16, 48)[0]
+    base = make(61, k, torch.bfloat16, 49)
+    x = base.repeat(-(-rows // 61), 1)[:rows]
+    y, s, h = rmsnorm_quant(x, w, 1e-5, residual=x, quant_dtype=torch.int8)
+    v, h64 = norm64(base, w, 1e-5, base)
+    assert torch.equal(h[-122:], h64[tail])
+    check(y[-122:], s[-122:], v[tail], torch.int8, norm_rel(k))
+    del x, y, s, h
+    base = make(61, 2 * k, torch.bfloat16, 50)
+    x = base.repeat(-(-rows // 61), 1)[:rows]
+    assert x.numel() > 2**32 and rows * k > 2**31
+    for quant in (FP8, None):
+        y, s = silu_mul_quant(x, quant_dtype=quant)
+        check(y[-122:], None if s is None else s[-122:], silu64(base)[tail], quant, SILU_REL)
+        del y, s

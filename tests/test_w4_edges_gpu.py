@@ -30,3 +30,14 @@ def test_more_tokens_than_a_grid_has_rows():
     compile_w4a16_gemv(N=n, K=k, group_size=32, zero_points=True)(c, a, q, s, z, None, m, n)
     assert bool((c[m:] == -77.0).all())
     check(c[:m], a, q, s, z, None, 32)
+
+
+@pytest.mark.parametrize("m", [1, 4, 8, 40])
+def test_weights_past_four_gigabytes(m):
+    n, k = 140001, 65536
+    a, q, s, z, _ = make(m, n, k, 128, "bf16", True, 13)
+    assert q.numel() > 2**32
+    c = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    compile_w4a16_gemv(N=n, K=k, zero_points=True)(c, a, q, s, z, None, m, n)
+    for part in (slice(0, 200), slice(n // 2, n // 2 + 200), slice(n - 200, n)):
+        check(c[:, part], a, q[part], s[part], z[part], None, 128)
