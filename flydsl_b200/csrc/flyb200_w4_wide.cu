@@ -10,7 +10,8 @@
 //
 // Bound: issue slots of the decoding.  13 instructions for 8 codes, 9 of them on the integer pipe (64 lanes a cycle and SM: 57 weights a
 // cycle, the stream at the copy rate is 46), and what moves, waits and sums around them: 16 x 18944 x 8192, where every SM has one
-// tile, takes 24.1 us (floor 12.2); 16 x 28672 x 8192, 1.5 tiles for an SM, 46.6.
+// tile, takes 24.1 us (floor 12.2); 16 x 28672 x 8192, 1.5 tiles for an SM, 47.5.  64 x 8192 x 28672, groups of 64: 61.6 on 128 blocks, 20 SMs without
+// one; on the others the integer pipe is 66 % and the issue slots 78 % busy.
 // Measured against it: the warp-level instruction on codes decoded in registers takes 57.5 us for 16 x 28672 x 8192, 154 for 32 tokens.
 #include "../../include/flyb200.h"
 #include "gemm_kernels.cuh"

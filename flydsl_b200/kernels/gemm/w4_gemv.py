@@ -14,7 +14,7 @@ and 128.  ``epilogue``, ``bias`` [N] and ``stream`` are those of ``compile_presh
 activations.  Sums are fp32 and no weight is rounded on the way: code minus zero point is exact, and the scale multiplies the
 sum of its group.  Up to 4 tokens the activations of a group are rounded to within 2^-22 of the group's largest magnitude (exact
 products and sums of integers); a token that holds an infinity or a NaN gives no finite number, and which of the two
-may depend on the number of tokens.
+may depend on the number of tokens.  So may the last places of a token's results: up to 4 tokens and from 5 on the sums differ in order.
 
 Any number of tokens runs, in blocks of 64 that each stream the weights; for more than that the 8-bit products
 on the tensor core (``compile_preshuffle_gemm``) are the faster ones.  Weights, activations and scales are read in place, on
@@ -48,7 +48,7 @@ def per_group_w4_quant(w: torch.Tensor, group_size: int = 128, *, zero_points: b
     """``(codes, scale, zero)`` of weights [N, K] as torch operations on their device.  Without zero points scale =
     max|w| / 7 over a group and zero is None; with them the group's range, which always holds 0, is spread over 0..15.  The
     codes are the nearest ones under the scale as it is stored (``scale_dtype``, by default w's own 16-bit type, bf16 for
-    fp32).  A group of zeros gets scale 1."""
+    fp32; it has to hold the scales: fp16 none beyond 65504).  A group of zeros gets scale 1."""
     if not isinstance(w, torch.Tensor) or w.dim() != 2 or not w.dtype.is_floating_point:
         raise ValueError("w must be a two-dimensional tensor of floating-point weights")
     if group_size not in GROUP_SIZES or w.shape[1] % group_size != 0 or w.numel() == 0:

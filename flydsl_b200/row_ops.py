@@ -190,7 +190,7 @@ def rmsnorm_quant(x, weight, eps=1e-6, *, residual=None, quant_dtype=torch.float
 
 def silu_mul_quant(x, *, quant_dtype=torch.float8_e4m3fn):
     """``(y, scale)``: codes and scales of ``silu(gate) * up`` for ``x = [..., 2 * inter]``, of every row the gate values
-    first (the row order of a gate-up projection's weights), values in fp32."""
+    first (the row order of a gate-up projection's weights), values in fp32 (to 2^-20 of themselves, for every gate)."""
     quant = _code(quant_dtype)
     if not torch.compiler.is_compiling():
         r = _lib.ops().silu_mul_quant(x, quant)
